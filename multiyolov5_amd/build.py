@@ -25,6 +25,8 @@ def stale():
 
 # augment.hip restates C code compiled for baseline x86-64 (Pillow / OpenCV float arithmetic): a fused multiply-add changes the
 # truncated uint8 results.  hipcc's default -ffp-contract=fast ignores source pragmas, so the whole file is built without contraction.
+# no v_pk_{add,mul,fma}_f32 anywhere: scalar fp32 instructions give the same IEEE results
+NO_PACKED_F32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 PER_FILE_FLAGS = {'augment.hip': ['-ffp-contract=off']}
 
 
@@ -43,14 +45,15 @@ def build(force=False, verbose=True):
         objs.append(obj)
         if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(src), hdr_t):
             continue                                     # object is newer than its source and every header
-        cmd = [hipcc, f'--offload-arch={ARCH}', '-O3', '-std=c++17', '-fPIC'] + PER_FILE_FLAGS.get(os.path.basename(src), []) + ['-c', src, '-o', obj]
+        cmd = [hipcc, f'--offload-arch={ARCH}', '-O3', '-std=c++17', '-fPIC'] + NO_PACKED_F32 + PER_FILE_FLAGS.get(os.path.basename(src), []) + ['-c', src, '-o', obj]
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     for cmd, p in procs:
         out, _ = p.communicate()
         if p.returncode != 0:
             raise RuntimeError('hipcc failed: %s\n%s' % (' '.join(cmd), out.decode()))
-        if verbose and out.strip():
-            print(out.decode())
+        text = '\n'.join(ln for ln in out.decode().splitlines() if 'packed-fp32-ops' not in ln)   # (the host pass does not know the feature)
+        if verbose and text.strip():
+            print(text)
     cmd = [hipcc, f'--offload-arch={ARCH}', '-shared', '-fPIC', '-o', LIB] + objs
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     if r.returncode != 0:
