@@ -404,6 +404,72 @@ int myolo_detect_unpermute(const void* g, int g_dtype, int na, int no, const myo
 int myolo_detect_decode(const void* raw, int dtype, int n, int na, int ny, int nx, int no, float stride,
                         const float* anchor_wh_px, void* z, int64_t a_total, int64_t row0, void* stream);
 
+/* ---- token operators: a feature map (or clip) as a sequence of pixel rows -------------------------------
+ * What a transformer layer over feature-map tokens needs next to the 1x1 convolutions (the reference's is models/common.py:49-92). */
+
+/* Layer norm over the channels of every pixel row: y = (x - mu) * rstd * gamma + beta, rstd = (mean (x - mu)^2 + eps)^-1/2; statistics in
+ * fp32.  x, out: views of one shape and dtype (any c >= 1, any strides; 16-byte aligned rows take the vector path); out may be x.
+ * gamma / beta: fp32[c] or NULL (1 / 0).  saved: fp32[2 * rows] (rows = n*h*w: the means, then the rstds) for the backward, or NULL. */
+int myolo_layernorm_fwd(const myolo_tensor* x, const float* gamma, const float* beta, float eps, const myolo_tensor* out, float* saved,
+                        void* stream);
+/* gx (+)= rstd * (g - mean g - xhat * mean(g * xhat)), g = gout * gamma;  dgamma (+)= sum_rows gout * xhat;  dbeta (+)= sum_rows gout.
+ * gx.ptr == NULL, dgamma == NULL, dbeta == NULL: that gradient is not wanted.  acc_x / acc_params: add to what gx / dgamma and dbeta hold.
+ * ws: myolo_layernorm_ws_bytes(rows, c) bytes of scratch, 16-byte aligned (needed when dgamma or dbeta is wanted); the sums are formed in
+ * a fixed order.  gx may be gout. */
+int64_t myolo_layernorm_ws_bytes(int64_t rows, int c);
+int myolo_layernorm_bwd(const myolo_tensor* gout, const myolo_tensor* x, const float* saved, const float* gamma, const myolo_tensor* gx,
+                        int acc_x, float* dgamma, float* dbeta, int acc_params, float* ws, int64_t ws_bytes, void* stream);
+
+/* Rotary positions with several axes: pair j (of npair <= MYOLO_ROPE_MAX_PAIRS) of every head is turned by
+ * 2 pi * turns[j] * pos[token][axis[j]]; channels behind the first 2*npair pass through.  Pair j is channels (j, j + npair), or
+ * (2j, 2j + 1) when interleaved.  The turn count is formed and reduced in fp64.  inverse = 1: the opposite angle (the backward).
+ * q [b, l, hq, d] and k [b, l, hk, d] share positions and launch; k == NULL (hk = 0): q alone.  qo / ko: the results; either is its
+ * input itself (same strides) or does not overlap any input.  Strides in elements: {batch, token, head}, pos {batch, token, axis};
+ * channel stride 1.  turns, axis: HOST arrays, read during the call. */
+#define MYOLO_ROPE_MAX_PAIRS 128
+#define MYOLO_ROPE_MAX_AXES 4
+typedef struct myolo_rope_desc {
+  const void *q, *k;
+  void *qo, *ko;
+  const int64_t* pos;
+  const double* turns;
+  const int32_t* axis;
+  int64_t qs[3], ks[3], qos[3], kos[3], ps[3];
+  int32_t b, l, hq, hk, d, npair, naxis, interleaved, inverse, dtype;
+} myolo_rope_desc;
+int myolo_rope(const myolo_rope_desc* d, void* stream);
+
+/* Attention with a sliding window and leading keys that stay visible.  q, o [b, lq, hq, d], k, v [b, lk, hk, d] (hq a multiple of hk: query
+ * head h reads key head h / (hq / hk)); element strides {batch, token, head}, channel stride 1.  d <= 128 and a multiple of 8, pointers
+ * and strides multiples of 16 bytes, lq, lk, window <= MYOLO_ATTN_MAX_LEN, anything else is MYOLO_EINVAL.
+ *   p = starts[b] + i  (starts == NULL: lk - lq + i) is query i's position;  key j is visible when  j < lens[b] (lens == NULL: lk)
+ *   and (not causal or j <= p) and (window == 0 or |p - j| < window or j < sinks)
+ *   o = softmax over the visible keys of scale * q.k, times v; a query that sees nothing gives 0.
+ * Keys that no query of the call sees are never read into a result, whatever they hold.  lens, starts: device int32[b].
+ * lse: fp32 [b, hq, lq] (log2 of the softmax denominator of scale*log2(e)*q.k), written by the forward when not NULL, read by the
+ * backward.  scale > 0.
+ * ws: myolo_attn_ws_bytes(d, backward) bytes of scratch, 16-byte aligned (0: none needed), free again when the call's work has run.
+ * Backward: go = d loss / d o; gq, gk, gv are overwritten (each may be NULL: not wanted; gk and gv are wanted together).  No atomics:
+ * results do not depend on the order in which workgroups run. */
+#define MYOLO_ATTN_MAX_LEN (1 << 28)
+typedef struct myolo_attn_desc {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;
+  const int32_t *lens, *starts;
+  const void* go;
+  void *gq, *gk, *gv;
+  void* ws;
+  int64_t ws_bytes;
+  int64_t qs[3], ks[3], vs[3], os[3], gos[3], gqs[3], gks[3], gvs[3];
+  int32_t b, lq, lk, hq, hk, d, dtype, causal, window, sinks;
+  float scale;
+  int32_t reserved;
+} myolo_attn_desc;
+int64_t myolo_attn_ws_bytes(const myolo_attn_desc* d, int backward);
+int myolo_attn_fwd(const myolo_attn_desc* d, void* stream);
+int myolo_attn_bwd(const myolo_attn_desc* d, void* stream);
+
 /* ---- losses ------------------------------------------------------------------------------------ */
 /* nn.CrossEntropyLoss(ignore_index) over [N,C,H,W]-logical logits with element strides (utils/loss.py:236-237).
  * acc (double[2], device): zeroed here, then acc[0] = sum of per-pixel losses, acc[1] = number of valid pixels.

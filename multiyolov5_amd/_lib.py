@@ -113,6 +113,29 @@ class TinyConvDesc(C.Structure):
                 ('gout', Tensor), ('dy', Tensor), ('gx', Tensor), ('dgamma', C.c_void_p), ('dbeta', C.c_void_p)]
 
 
+class RopeDesc(C.Structure):
+    """myolo_rope_desc (include/myolo.h)"""
+    _fields_ = [('q', C.c_void_p), ('k', C.c_void_p), ('qo', C.c_void_p), ('ko', C.c_void_p), ('pos', C.c_void_p), ('turns', C.c_void_p),
+                ('axis', C.c_void_p), ('qs', C.c_int64 * 3), ('ks', C.c_int64 * 3), ('qos', C.c_int64 * 3), ('kos', C.c_int64 * 3),
+                ('ps', C.c_int64 * 3), ('b', C.c_int32), ('l', C.c_int32), ('hq', C.c_int32), ('hk', C.c_int32), ('d', C.c_int32),
+                ('npair', C.c_int32), ('naxis', C.c_int32), ('interleaved', C.c_int32), ('inverse', C.c_int32), ('dtype', C.c_int32)]
+
+
+ROPE_MAX_PAIRS, ROPE_MAX_AXES = 128, 4      # MYOLO_ROPE_MAX_PAIRS, MYOLO_ROPE_MAX_AXES
+
+
+class AttnDesc(C.Structure):
+    """myolo_attn_desc (include/myolo.h)"""
+    _fields_ = [('q', C.c_void_p), ('k', C.c_void_p), ('v', C.c_void_p), ('o', C.c_void_p), ('lse', C.c_void_p), ('lens', C.c_void_p),
+                ('starts', C.c_void_p), ('go', C.c_void_p), ('gq', C.c_void_p), ('gk', C.c_void_p), ('gv', C.c_void_p), ('ws', C.c_void_p),
+                ('ws_bytes', C.c_int64), ('qs', C.c_int64 * 3), ('ks', C.c_int64 * 3), ('vs', C.c_int64 * 3), ('os', C.c_int64 * 3),
+                ('gos', C.c_int64 * 3), ('gqs', C.c_int64 * 3), ('gks', C.c_int64 * 3), ('gvs', C.c_int64 * 3),
+                ('b', C.c_int32), ('lq', C.c_int32), ('lk', C.c_int32), ('hq', C.c_int32), ('hk', C.c_int32), ('d', C.c_int32),
+                ('dtype', C.c_int32), ('causal', C.c_int32), ('window', C.c_int32), ('sinks', C.c_int32), ('scale', C.c_float),
+                ('reserved', C.c_int32)]
+
+
+ATTN_MAX_LEN = 1 << 28      # MYOLO_ATTN_MAX_LEN
 TINY_MAX_PIX, TINY_MAX_GROUP = 1024, 4      # MYOLO_TINY_MAX_PIX, MYOLO_TINY_MAX_GROUP
 
 
@@ -164,6 +187,13 @@ _PROTOS = {
     'myolo_gate_bwd': (C.c_int, [TP, TP, TP, TP, C.c_int, P, P]),
     'myolo_gate_mul_fwd': (C.c_int, [TP, TP, TP, P]),
     'myolo_gate_mul_bwd': (C.c_int, [TP, TP, TP, TP, C.c_int, P, P]),
+    'myolo_layernorm_fwd': (C.c_int, [TP, P, P, C.c_float, TP, P, P]),
+    'myolo_layernorm_ws_bytes': (C.c_int64, [C.c_int64, C.c_int]),
+    'myolo_layernorm_bwd': (C.c_int, [TP, TP, P, P, TP, C.c_int, P, P, C.c_int, P, C.c_int64, P]),
+    'myolo_rope': (C.c_int, [C.POINTER(RopeDesc), P]),
+    'myolo_attn_ws_bytes': (C.c_int64, [C.POINTER(AttnDesc), C.c_int]),
+    'myolo_attn_fwd': (C.c_int, [C.POINTER(AttnDesc), P]),
+    'myolo_attn_bwd': (C.c_int, [C.POINTER(AttnDesc), P]),
     'myolo_add': (C.c_int, [TP, TP, C.c_int, P]),
     'myolo_fill_zero': (C.c_int, [TP, P]),
     'myolo_cast_from_f32': (C.c_int, [P, TP, P]),

@@ -1,0 +1,738 @@
+// Attention with a sliding window and leading keys that stay visible (sinks): forward, split over the key axis for few rows, backward.
+//
+//   S = scale q k^T over the visible keys, P = softmax(S), o = P v
+//   dP = do v^T,  delta = rowsum(do * o),  dS = P (dP - delta);   dq = scale dS k,  dk = scale dS^T q,  dv = P^T do
+//
+// All products run on the 32x32 matrix instruction with the score tile transposed as its consumer needs it: a lane of the result holds ONE
+// column (lane % 32) and 16 rows 8*(r/4) + r%4 + 4*(lane/32).  The forward and dq form S^T = K Q^T, so that a lane owns one query: the
+// softmax statistics stay in the lane (one exchange between the wave's halves per tile) and the 16 keys it holds are, in this order, the
+// contraction operand of O^T = V^T P^T -- no shuffle of P.  dk / dv form S = Q K^T for the same reason with the key in the lane.  The other
+// operand of the second product is read across the rows of its LDS tile: transposing 8-byte LDS reads for fp16, plain reads for fp32 (whose
+// 8-element operands feed eight 32x32x2 instructions).
+// The rows of a (batch, key head) are its query heads' queries, i * group + g: one K / V tile serves all heads of the group.
+#include "myolo_dev.h"
+
+namespace {
+
+typedef float f16_t __attribute__((ext_vector_type(16)));
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnArgs {
+  const char *q, *k, *v, *go;
+  char *o, *gq, *gk, *gv;
+  float *lse, *delta;
+  float* part;             // split forward: [split][b*hk][rows][d] unnormalised sums, then [split][b*hk][rows][2] max and denominator
+  const int *lens, *starts;
+  int64_t qs[3], ks[3], vs[3], os[3], gos[3], gqs[3], gks[3], gvs[3];      // bytes
+  int b, lq, lk, hq, hk, g, d, causal, window, sinks;
+  int rows, nblk, nsplit;
+  float scale, sl2;        // scale, scale * log2(e)
+};
+
+// ---- fragments: 8 elements along the contracted axis --------------------------------------------------------------------------------
+template <typename T> struct Frag;
+template <> struct Frag<half_t> { h8_t v; };
+template <> struct Frag<float> { f4_t a, b; };
+
+__device__ __forceinline__ f16_t mma(const Frag<half_t>& a, const Frag<half_t>& b, f16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16_t mma(const Frag<float>& a, const Frag<float>& b, f16_t c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.a[i], b.a[i], c, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.b[i], b.b[i], c, 0, 0, 0);
+  return c;
+}
+// 8 accumulator registers 8*S .. 8*S + 7 as an operand
+template <int S> __device__ __forceinline__ void frag_from(Frag<half_t>& f, const f16_t& c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f.v[i] = (half_t)c[8 * S + i];
+}
+template <int S> __device__ __forceinline__ void frag_from(Frag<float>& f, const f16_t& c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f.a[i] = c[8 * S + i]; f.b[i] = c[8 * S + 4 + i]; }
+}
+// 8 consecutive elements of a row in global memory, zeros where !ok
+__device__ __forceinline__ void frag_global(Frag<half_t>& f, const char* p, bool ok) {
+  const uint4 v = ldg16(ok ? p : zero_page());
+  f.v = *reinterpret_cast<const h8_t*>(&v);
+}
+__device__ __forceinline__ void frag_global(Frag<float>& f, const char* p, bool ok) {
+  const uint4 v = ldg16(ok ? p : zero_page()), w = ldg16(ok ? p + 16 : zero_page());
+  f.a = *reinterpret_cast<const f4_t*>(&v);
+  f.b = *reinterpret_cast<const f4_t*>(&w);
+}
+__device__ __forceinline__ float frag_dot(const Frag<half_t>& a, const Frag<half_t>& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += (float)a.v[i] * (float)b.v[i];
+  return s;
+}
+__device__ __forceinline__ float frag_dot(const Frag<float>& a, const Frag<float>& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s += a.a[i] * b.a[i] + a.b[i] * b.b[i];
+  return s;
+}
+
+// ---- LDS tiles: rows of DL elements in 16-byte chunks; chunk c of row r sits at c ^ swz(r), so that 16 rows at one chunk (row operands) and 4
+// rows x 4 chunks (transposing reads) both cover all 64 banks
+template <typename T, int DL> struct Tile {
+  static constexpr int EC = 16 / (int)sizeof(T);            // elements a chunk
+  static constexpr int CH = DL / EC;                        // chunks a row
+  __device__ static __forceinline__ int swz(int r) {
+    if constexpr (CH >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (CH == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+  }
+  __device__ static __forceinline__ int unit(int r, int c) { return r * CH + (c ^ swz(r)); }
+  // row operand: 8 elements at column 8*c8 of row r
+  __device__ static __forceinline__ void row_frag(Frag<half_t>& f, const uint4* s, int r, int c8) {
+    f.v = *reinterpret_cast<const h8_t*>(s + unit(r, c8));
+  }
+  __device__ static __forceinline__ void row_frag(Frag<float>& f, const uint4* s, int r, int c8) {
+    f.a = *reinterpret_cast<const f4_t*>(s + unit(r, 2 * c8));
+    f.b = *reinterpret_cast<const f4_t*>(s + unit(r, 2 * c8 + 1));
+  }
+  // column operand: column c0 + lane % 32, rows r0 + {0..3, 8..11} + 4 * (lane / 32)
+  __device__ static __forceinline__ void col_frag(Frag<half_t>& f, const uint4* s, int r0, int c0, int lane) {
+    typedef __attribute__((address_space(3))) fp16x4_t lds_t;
+    const int sub = lane & 15;
+    const int c = (c0 >> 3) + ((lane >> 4) & 1) * 2 + ((sub & 3) >> 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = r0 + 8 * i + 4 * (lane >> 5) + (sub >> 2);
+      const char* p = reinterpret_cast<const char*>(s + unit(r, c)) + (sub & 1) * 8;
+      const fp16x4_t t = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_t*)(p));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f.v[4 * i + e] = (half_t)t[e];
+    }
+  }
+  __device__ static __forceinline__ void col_frag(Frag<float>& f, const uint4* s, int r0, int c0, int lane) {
+    const int col = c0 + (lane & 31);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = r0 + 4 * (lane >> 5) + e;
+      f.a[e] = reinterpret_cast<const float*>(s + unit(r, col >> 2))[col & 3];
+      f.b[e] = reinterpret_cast<const float*>(s + unit(r + 8, col >> 2))[col & 3];
+    }
+  }
+};
+
+// the value of the lane's column in the other half of the wave, combined
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- what is visible -----------------------------------------------------------------------------------------------------------------
+struct Vis {
+  int start, len, causal, window, sinks;
+  __device__ __forceinline__ bool sees(int p, int j) const {
+    const int dist = p > j ? p - j : j - p;
+    return j < len && (!causal || j <= p) && (!window || dist < window || j < sinks);
+  }
+  // every query of positions [p0, p1] sees every key of [j0, j1]
+  __device__ __forceinline__ bool all(int p0, int p1, int j0, int j1) const {
+    return j1 < len && (!causal || j1 <= p0) && (!window || (p1 - j0 < window && j1 - p0 < window) || j1 < sinks);
+  }
+  // some query of [p0, p1] may see some key of [j0, j1]
+  __device__ __forceinline__ bool any(int p0, int p1, int j0, int j1) const {
+    return j0 < len && (!causal || j0 <= p1) && (!window || (p0 - j1 < window && j0 - p1 < window) || j0 < sinks);
+  }
+  // some query of [p0, p1] sees key j (exact: positions are consecutive)
+  __device__ __forceinline__ bool key(int p0, int p1, int j) const { return j >= 0 && any(p0, p1, j, j); }
+};
+// (start is clamped to where nothing changes any more, so that positions and distances stay within 32 bits: all lengths <= 2^28)
+__device__ __forceinline__ Vis vis_of(const AttnArgs& a, int b) {
+  Vis v{a.lk - a.lq, a.lk, a.causal, a.window, a.sinks};
+  if (a.lens) v.len = min(max(a.lens[b], 0), a.lk);
+  if (a.starts) v.start = min(max(a.starts[b], -a.lq - a.window), a.lk + a.window);
+  return v;
+}
+// the key tiles of BK that queries [p0, p1] may see: tiles [0, n1) hold sinks only, n - n1 tiles from lo on the band
+struct TileList { int n1, lo, n; __device__ __forceinline__ int at(int i) const { return i < n1 ? i : lo + (i - n1); } };
+__device__ __forceinline__ TileList tiles_of(const Vis& v, int p0, int p1, int bk) {
+  int hi = v.causal ? min(v.len, p1 + 1) : v.len, lo = 0, first = 0;
+  if (v.window) {
+    first = max(0, min(v.sinks, hi));                       // keys [0, first) stay visible
+    lo = max(0, p0 - v.window + 1);
+    hi = min(hi, p1 + v.window);
+    if (hi <= lo) hi = lo = 0;                              // an empty band
+    if (first >= lo) { lo = 0; hi = max(hi, first); first = 0; }       // one run of keys
+  }
+  const int tlo = lo / bk, thi = max((max(hi, 0) + bk - 1) / bk, tlo), n1 = min((first + bk - 1) / bk, tlo);
+  return TileList{n1, tlo, n1 + thi - tlo};
+}
+
+// ROWS x DP elements from global rows into registers (zeros for hidden rows and channels >= d), registers into a tile
+template <typename T, int DP, int ROWS, int NT> struct Stage {
+  static constexpr int EC = 16 / (int)sizeof(T), CH = DP / EC, N = ROWS * CH, PER = (N + NT - 1) / NT;
+  uint4 v[PER];
+  template <class F> __device__ __forceinline__ void load(const char* base, int64_t stride, int d, int tid, F row_ok) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = tid + i * NT, r = u / CH, c = u - r * CH;
+      const bool ok = u < N && c * EC < d && row_ok(r);
+      v[i] = ldg16(ok ? base + (int64_t)r * stride + c * 16 : zero_page());
+    }
+  }
+  template <int DL> __device__ __forceinline__ void store(uint4* s, int tid) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = tid + i * NT, r = u / CH, c = u - r * CH;
+      if (N % NT == 0 || u < N) s[Tile<T, DL>::unit(r, c)] = v[i];
+    }
+  }
+};
+
+__host__ __device__ constexpr int lds_width(int dp) { return dp <= 32 ? 32 : dp <= 64 ? 64 : 128; }
+
+// consecutive workgroups go round the 8 XCDs: give each XCD a contiguous run of the work, so that neighbours share K / V in its L2
+__device__ __forceinline__ int xcd_order(int id, int n) {
+  const int per = n >> 3, rem = n & 7, x = id & 7, k = id >> 3;
+  return x * per + min(x, rem) + k;
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP, int NW, bool SPLIT>
+__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
+  constexpr int BK = sizeof(T) == 2 || NW > 1 ? 64 : 32, U = BK / 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
+  using TL = Tile<T, DL>;
+  __shared__ uint4 sK[BK * TL::CH], sV[BK * TL::CH];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+  int id = xcd_order(blockIdx.x, gridDim.x);
+  const int sp = SPLIT ? id % a.nsplit : 0;
+  if (SPLIT) id /= a.nsplit;
+  const int blk = a.nblk - 1 - id % a.nblk, bh = id / a.nblk;       // (long causal blocks first)
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const Vis vis = vis_of(a, b);
+  const int r0 = blk * 32 * NW, r1 = min(r0 + 32 * NW, a.rows) - 1;
+  const int pb0 = vis.start + r0 / a.g, pb1 = vis.start + r1 / a.g;
+  const int w0 = min(r0 + wv * 32, r1), w1 = min(w0 + 31, r1);
+  const int pw0 = vis.start + w0 / a.g, pw1 = vis.start + w1 / a.g;
+  const int row = r0 + wv * 32 + (lane & 31);
+  const bool live = row < a.rows;
+  const int qi = (live ? row : r1) / a.g, head = kh * a.g + (live ? row : r1) - qi * a.g;
+  const int p = vis.start + qi;
+
+  Frag<T> qf[KS];
+  const char* qp = a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) frag_global(qf[s], qp + (s * 16 + h * 8) * sizeof(T), live && s * 16 + h * 8 < a.d);
+
+  const char* kp = a.k + b * a.ks[0] + kh * a.ks[2];
+  const char* vp = a.v + b * a.vs[0] + kh * a.vs[2];
+  f16_t o[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) o[m] = f16_t{};
+  float mx = -INFINITY, l = 0.f;
+
+  const TileList tl = tiles_of(vis, pb0, pb1, BK);
+  int t0 = 0, t1 = tl.n;
+  if (SPLIT) {
+    const int per = (tl.n + a.nsplit - 1) / a.nsplit;
+    t0 = min(sp * per, tl.n);
+    t1 = min(t0 + per, tl.n);
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int j0 = tl.at(t) * BK;
+    {
+      Stage<T, DP, BK, NT> gk, gv;
+      auto ok = [&](int r) { return vis.key(pb0, pb1, j0 + r); };
+      gk.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.d, tid, ok);
+      gv.load(vp + (int64_t)j0 * a.vs[1], a.vs[1], a.d, tid, ok);
+      __syncthreads();
+      gk.template store<DL>(sK, tid);
+      gv.template store<DL>(sV, tid);
+      __syncthreads();
+    }
+    if (!vis.any(pw0, pw1, j0, j0 + BK - 1)) continue;
+    f16_t s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s[u] = f16_t{};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        Frag<T> kf;
+        TL::row_frag(kf, sK, u * 32 + (lane & 31), k * 2 + h);
+        s[u] = mma(kf, qf[k], s[u]);
+      }
+    }
+    if (!vis.all(pw0, pw1, j0, j0 + BK - 1)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!vis.sees(p, j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h)) s[u][r] = -INFINITY;
+    }
+    float m2 = s[0][0];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m2 = fmaxf(m2, s[u][r]);
+    m2 = fmaxf(mx, half_max(m2) * a.sl2);
+    const float use = m2 == -INFINITY ? 0.f : m2;
+    const float al = __builtin_amdgcn_exp2f(mx - use);
+    mx = m2;
+    float ls = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.sl2, -use));
+        ls += s[u][r];
+      }
+    l = l * al + ls;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[m][r] *= al;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Frag<T> p0, p1, vf;
+      frag_from<0>(p0, s[u]);
+      frag_from<1>(p1, s[u]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        TL::col_frag(vf, sV, u * 32, m * 32, lane);
+        o[m] = mma(vf, p0, o[m]);
+        TL::col_frag(vf, sV, u * 32 + 16, m * 32, lane);
+        o[m] = mma(vf, p1, o[m]);
+      }
+    }
+  }
+  l = half_sum(l);
+  if (!live) return;
+  if (SPLIT) {
+    const int64_t pr = ((int64_t)sp * (a.b * a.hk) + bh) * a.rows + row;
+    float* po = a.part + pr * a.d;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int c = m * 32 + q4 * 8 + 4 * h;
+        if (c < a.d) *reinterpret_cast<f4_t*>(po + c) = f4_t{o[m][4 * q4], o[m][4 * q4 + 1], o[m][4 * q4 + 2], o[m][4 * q4 + 3]};
+      }
+    if (h == 0) {
+      float* ml = a.part + (int64_t)a.nsplit * (a.b * a.hk) * a.rows * a.d + pr * 2;
+      ml[0] = mx;
+      ml[1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (a.lse && h == 0) a.lse[((int64_t)b * a.hq + head) * a.lq + qi] = l == 0.f ? -INFINITY : mx + __log2f(l);
+  char* op = a.o + b * a.os[0] + qi * a.os[1] + head * a.os[2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int c = m * 32 + q4 * 8 + 4 * h;
+      if (c >= a.d) continue;
+      if constexpr (sizeof(T) == 2) {
+        h4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (half_t)(o[m][4 * q4 + e] * inv);
+        *reinterpret_cast<h4_t*>(op + c * 2) = v;
+      } else {
+        f4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = o[m][4 * q4 + e] * inv;
+        *reinterpret_cast<f4_t*>(op + c * 4) = v;
+      }
+    }
+}
+
+// joins the splits of a row: o = sum o_s 2^(m_s - M) / sum l_s 2^(m_s - M)
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  const int64_t nrow = (int64_t)a.b * a.hk * a.rows, total = nrow * (a.d / 4);
+  const float* ml = a.part + (int64_t)a.nsplit * nrow * a.d;
+  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
+    const int64_t pr = v / (a.d / 4);
+    const int c = (int)(v - pr * (a.d / 4)) * 4;
+    float mx = -INFINITY;
+    for (int s = 0; s < a.nsplit; ++s) mx = fmaxf(mx, ml[(s * nrow + pr) * 2]);
+    const float use = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f;
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.nsplit; ++s) {
+      const float w = __builtin_amdgcn_exp2f(ml[(s * nrow + pr) * 2] - use);
+      l += w * ml[(s * nrow + pr) * 2 + 1];
+      const f4_t x = *reinterpret_cast<const f4_t*>(a.part + (s * nrow + pr) * a.d + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += w * x[e];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int bh = (int)(pr / a.rows), row = (int)(pr - (int64_t)bh * a.rows), b = bh / a.hk;
+    const int qi = row / a.g, head = (bh - b * a.hk) * a.g + row - qi * a.g;
+    if (a.lse && c == 0) a.lse[((int64_t)b * a.hq + head) * a.lq + qi] = l == 0.f ? -INFINITY : mx + __log2f(l);
+    T* op = (T*)(a.o + b * a.os[0] + qi * a.os[1] + head * a.os[2]) + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) op[e] = (T)(o[e] * inv);
+  }
+}
+
+// ---- backward: dq (and delta) --------------------------------------------------------------------------------------------------------
+// P enters the fp16 products times 2^12: a probability below 6e-5 (rows of more than 2^14 keys) would lose bits as an fp16 subnormal
+constexpr float kPShift = 12.f, kPUnshift = 1.f / 4096.f;
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_bwd_q_kernel(AttnArgs a) {
+  constexpr int NW = 4, BK = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
+  using TL = Tile<T, DL>;
+  __shared__ uint4 sK[BK * TL::CH], sV[BK * TL::CH];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  const int blk = a.nblk - 1 - id % a.nblk, bh = id / a.nblk;
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const Vis vis = vis_of(a, b);
+  const int r0 = blk * 32 * NW, r1 = min(r0 + 32 * NW, a.rows) - 1;
+  const int pb0 = vis.start + r0 / a.g, pb1 = vis.start + r1 / a.g;
+  const int w0 = min(r0 + wv * 32, r1), w1 = min(w0 + 31, r1);
+  const int pw0 = vis.start + w0 / a.g, pw1 = vis.start + w1 / a.g;
+  const int row = r0 + wv * 32 + (lane & 31);
+  const bool live = row < a.rows;
+  const int qi = (live ? row : r1) / a.g, head = kh * a.g + (live ? row : r1) - qi * a.g;
+  const int p = vis.start + qi;
+
+  Frag<T> qf[KS], gf[KS];
+  const char* qp = a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
+  const char* gp = a.go + b * a.gos[0] + qi * a.gos[1] + head * a.gos[2];
+  const char* op = a.o + b * a.os[0] + qi * a.os[1] + head * a.os[2];
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int c = (s * 16 + h * 8);
+    const bool ok = live && c < a.d;
+    Frag<T> of;
+    frag_global(qf[s], qp + c * sizeof(T), ok);
+    frag_global(gf[s], gp + c * sizeof(T), ok);
+    frag_global(of, op + c * sizeof(T), ok);
+    delta += frag_dot(gf[s], of);
+  }
+  delta = half_sum(delta);
+  const int64_t lrow = ((int64_t)b * a.hq + head) * a.lq + qi;
+  const float lse = a.lse[lrow];
+  if (live && h == 0) a.delta[lrow] = delta;
+  const char* kp = a.k + b * a.ks[0] + kh * a.ks[2];
+  const char* vp = a.v + b * a.vs[0] + kh * a.vs[2];
+  f16_t dq[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) dq[m] = f16_t{};
+
+  const TileList tl = tiles_of(vis, pb0, pb1, BK);
+  for (int t = 0; a.gq && t < tl.n; ++t) {
+    const int j0 = tl.at(t) * BK;
+    {
+      Stage<T, DP, BK, NT> gk, gv;
+      auto ok = [&](int r) { return vis.key(pb0, pb1, j0 + r); };
+      gk.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.d, tid, ok);
+      gv.load(vp + (int64_t)j0 * a.vs[1], a.vs[1], a.d, tid, ok);
+      __syncthreads();
+      gk.template store<DL>(sK, tid);
+      gv.template store<DL>(sV, tid);
+      __syncthreads();
+    }
+    if (!vis.any(pw0, pw1, j0, j0 + BK - 1)) continue;
+    const bool all = vis.all(pw0, pw1, j0, j0 + BK - 1);
+#pragma unroll
+    for (int u = 0; u < BK / 32; ++u) {
+      f16_t s = f16_t{}, dp = f16_t{};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        Frag<T> f;
+        TL::row_frag(f, sK, u * 32 + (lane & 31), k * 2 + h);
+        s = mma(f, qf[k], s);
+        TL::row_frag(f, sV, u * 32 + (lane & 31), k * 2 + h);
+        dp = mma(f, gf[k], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, -lse)) * (dp[r] - delta);
+        s[r] = all || vis.sees(p, j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? x : 0.f;
+      }
+      Frag<T> d0, d1, kf;
+      frag_from<0>(d0, s);
+      frag_from<1>(d1, s);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        TL::col_frag(kf, sK, u * 32, m * 32, lane);
+        dq[m] = mma(kf, d0, dq[m]);
+        TL::col_frag(kf, sK, u * 32 + 16, m * 32, lane);
+        dq[m] = mma(kf, d1, dq[m]);
+      }
+    }
+  }
+  if (!live || !a.gq) return;
+  char* dp = a.gq + b * a.gqs[0] + qi * a.gqs[1] + head * a.gqs[2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int c = m * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
+      if (c < a.d) reinterpret_cast<T*>(dp)[c] = (T)(dq[m][r] * a.scale);
+    }
+}
+
+// ---- backward: dk, dv ----------------------------------------------------------------------------------------------------------------
+// a wave owns 32 keys (operands and both accumulators in registers), the workgroup's four waves walk the queries that may see its 128 keys
+// and, for each, the heads of the group: the gradient of a shared head is one sum in one place
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_bwd_kv_kernel(AttnArgs a) {
+  constexpr int NW = 4, BQ = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
+  using TL = Tile<T, DL>;
+  __shared__ uint4 sQ[BQ * TL::CH], sG[BQ * TL::CH];
+  __shared__ float sL[BQ], sD[BQ];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  const int blk = id % a.nblk, bh = id / a.nblk;
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const Vis vis = vis_of(a, b);
+  const int k0 = blk * 32 * NW, k1 = min(k0 + 32 * NW, a.lk) - 1;
+  const int kw0 = k0 + wv * 32, kw1 = min(kw0 + 31, a.lk - 1);
+  const int key = kw0 + (lane & 31);
+  const bool live = key < a.lk, seen = key < vis.len;
+
+  Frag<T> kf[KS], vf[KS];
+  const char* kp = a.k + b * a.ks[0] + kh * a.ks[2] + (int64_t)key * a.ks[1];
+  const char* vp = a.v + b * a.vs[0] + kh * a.vs[2] + (int64_t)key * a.vs[1];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int c = s * 16 + h * 8;
+    frag_global(kf[s], kp + c * sizeof(T), seen && c < a.d);
+    frag_global(vf[s], vp + c * sizeof(T), seen && c < a.d);
+  }
+  f16_t dk[MT], dv[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) dk[m] = dv[m] = f16_t{};
+
+  // queries that may see a key of [k0, k1]: positions [plo, phi]
+  int ilo = 0, ihi = a.lq - 1;
+  if (k0 >= vis.len) ihi = -1;
+  if (vis.causal) ilo = max(ilo, k0 - vis.start);
+  if (vis.window && k0 >= vis.sinks) {
+    ihi = min(ihi, k1 + vis.window - 1 - vis.start);
+    ilo = max(ilo, k0 - vis.window + 1 - vis.start);
+  }
+  for (int hd = 0; hd < a.g; ++hd) {
+    const int head = kh * a.g + hd;
+    const char* qp = a.q + b * a.qs[0] + head * a.qs[2];
+    const char* gp = a.go + b * a.gos[0] + head * a.gos[2];
+    const int64_t lrow = ((int64_t)b * a.hq + head) * a.lq;
+    for (int i0 = ilo / BQ * BQ; i0 <= ihi; i0 += BQ) {
+      {
+        // rows behind the last query and rows that see nothing (lse = -inf) enter as zeros
+        Stage<T, DP, BQ, NT> gq, gg;
+        auto ok = [&](int r) { return i0 + r < a.lq && a.lse[lrow + i0 + r] != -INFINITY; };
+        gq.load(qp + (int64_t)i0 * a.qs[1], a.qs[1], a.d, tid, ok);
+        gg.load(gp + (int64_t)i0 * a.gos[1], a.gos[1], a.d, tid, ok);
+        float ls = -INFINITY, de = 0.f;
+        if (tid < BQ && i0 + tid < a.lq) {
+          ls = a.lse[lrow + i0 + tid];
+          de = a.delta[lrow + i0 + tid];
+        }
+        __syncthreads();
+        gq.template store<DL>(sQ, tid);
+        gg.template store<DL>(sG, tid);
+        if (tid < BQ) {
+          sL[tid] = kPShift - ls;
+          sD[tid] = ls == -INFINITY ? 0.f : de * kPUnshift;
+        }
+        __syncthreads();
+      }
+      const int p0 = vis.start + i0, p1 = p0 + BQ - 1;
+      if (kw0 > kw1 || !vis.any(p0, p1, kw0, kw1)) continue;
+      const bool all = kw0 + 31 < a.lk && i0 + BQ <= a.lq && vis.all(p0, p1, kw0, kw1);
+#pragma unroll
+      for (int u = 0; u < BQ / 32; ++u) {
+        f16_t s = f16_t{}, dp = f16_t{};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          Frag<T> f;
+          TL::row_frag(f, sQ, u * 32 + (lane & 31), k * 2 + h);
+          s = mma(f, kf[k], s);
+          TL::row_frag(f, sG, u * 32 + (lane & 31), k * 2 + h);
+          dp = mma(f, vf[k], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int q = u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, sL[q]));
+          const bool on = all || (i0 + q < a.lq && sL[q] != INFINITY && live && vis.sees(p0 + q, key));
+          s[r] = on ? x : 0.f;
+          dp[r] = on ? x * fmaf(dp[r], kPUnshift, -sD[q]) : 0.f;
+        }
+        Frag<T> f0, f1, c;
+        frag_from<0>(f0, s);
+        frag_from<1>(f1, s);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          TL::col_frag(c, sG, u * 32, m * 32, lane);
+          dv[m] = mma(f0, c, dv[m]);
+          TL::col_frag(c, sG, u * 32 + 16, m * 32, lane);
+          dv[m] = mma(f1, c, dv[m]);
+        }
+        frag_from<0>(f0, dp);
+        frag_from<1>(f1, dp);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          TL::col_frag(c, sQ, u * 32, m * 32, lane);
+          dk[m] = mma(f0, c, dk[m]);
+          TL::col_frag(c, sQ, u * 32 + 16, m * 32, lane);
+          dk[m] = mma(f1, c, dk[m]);
+        }
+      }
+    }
+  }
+  // accumulators: column (lane % 32) = channel, rows = keys
+  const int col = lane & 31;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int kk = kw0 + (r & 3) + 8 * (r >> 2) + 4 * h;
+      if (kk < a.lk && m * 32 + col < a.d) {
+        reinterpret_cast<T*>(a.gk + b * a.gks[0] + kh * a.gks[2] + (int64_t)kk * a.gks[1])[m * 32 + col] = (T)(dk[m][r] * a.scale);
+        reinterpret_cast<T*>(a.gv + b * a.gvs[0] + kh * a.gvs[2] + (int64_t)kk * a.gvs[1])[m * 32 + col] = (T)(dv[m][r] * kPUnshift);
+      }
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------------
+bool desc_ok(const myolo_attn_desc* d) {
+  return d && (d->dtype == MYOLO_F16 || d->dtype == MYOLO_F32) && d->b >= 0 && d->lq >= 0 && d->lk >= 0 && d->lq <= MYOLO_ATTN_MAX_LEN &&
+         d->lk <= MYOLO_ATTN_MAX_LEN && d->hq >= 1 && d->hk >= 1 && d->hq % d->hk == 0 && d->d >= 8 && d->d <= 128 && d->d % 8 == 0 &&
+         d->window >= 0 && d->window <= MYOLO_ATTN_MAX_LEN && d->sinks >= 0 && (int64_t)d->b * d->hq < (1 << 24) &&
+         (int64_t)d->lq * (d->hq / d->hk) <= MYOLO_ATTN_MAX_LEN;
+}
+bool side_ok(const void* p, const int64_t* s, int es) {
+  if (!p || (uintptr_t)p % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (s[i] * es % 16) return false;
+  return true;
+}
+struct FwdShape { int nw, nblk, nsplit; };
+FwdShape fwd_shape(const myolo_attn_desc* d) {
+  const int64_t rows = (int64_t)d->lq * (d->hq / d->hk), bh = (int64_t)d->b * d->hk;
+  FwdShape f;
+  f.nw = rows > 32 ? 4 : 1;
+  f.nblk = (int)((rows + 32 * f.nw - 1) / (32 * f.nw));
+  // few workgroups over a long key axis: split it until there is work for four waves on every CU, a split keeping a tile at least
+  int64_t span = d->lk;
+  if (d->window) {
+    const int64_t w = (int64_t)d->window * (d->causal ? 1 : 2) + d->sinks + 32 * f.nw / (d->hq / d->hk) + 128;
+    if (w < span) span = w;
+  }
+  const int64_t tiles = (span + 63) / 64, want = 1024 / f.nw, have = bh * f.nblk;
+  int64_t n = have > 0 ? want / have : 1;
+  if (n > tiles) n = tiles;
+  if (n > 64) n = 64;
+  f.nsplit = n < 2 ? 1 : (int)n;
+  return f;
+}
+void bytes3(int64_t* o, const int64_t* s, int64_t es) { for (int i = 0; i < 3; ++i) o[i] = s[i] * es; }
+AttnArgs args_of(const myolo_attn_desc* d) {
+  const int64_t es = d->dtype == MYOLO_F16 ? 2 : 4;
+  AttnArgs a{};
+  a.q = (const char*)d->q; a.k = (const char*)d->k; a.v = (const char*)d->v; a.o = (char*)d->o; a.go = (const char*)d->go;
+  a.gq = (char*)d->gq; a.gk = (char*)d->gk; a.gv = (char*)d->gv;
+  a.lse = d->lse; a.lens = d->lens; a.starts = d->starts;
+  bytes3(a.qs, d->qs, es); bytes3(a.ks, d->ks, es); bytes3(a.vs, d->vs, es); bytes3(a.os, d->os, es);
+  bytes3(a.gos, d->gos, es); bytes3(a.gqs, d->gqs, es); bytes3(a.gks, d->gks, es); bytes3(a.gvs, d->gvs, es);
+  a.b = d->b; a.lq = d->lq; a.lk = d->lk; a.hq = d->hq; a.hk = d->hk; a.g = d->hq / d->hk; a.d = d->d;
+  a.causal = d->causal ? 1 : 0; a.window = d->window; a.sinks = d->sinks < d->lk ? d->sinks : d->lk;
+  a.rows = d->lq * a.g; a.nsplit = 1;
+  a.scale = d->scale; a.sl2 = d->scale * kLog2e;
+  return a;
+}
+
+template <typename T, int DP, int NW>
+int launch_fwd(const AttnArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.b * a.hk * a.nblk * a.nsplit));
+  if (a.nsplit > 1) {
+    hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, true>), grid, dim3(NW * 64), 0, st, a);
+    MYOLO_CHECK_LAUNCH();
+    const int64_t total = (int64_t)a.b * a.hk * a.rows * (a.d / 4);
+    hipLaunchKernelGGL((attn_join_kernel<T>), dim3(grid_for(total, 256, 4096)), dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, false>), grid, dim3(NW * 64), 0, st, a);
+  }
+  MYOLO_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T, int DP> int launch_fwd_w(const AttnArgs& a, int nw, hipStream_t st) {
+  return nw == 4 ? launch_fwd<T, DP, 4>(a, st) : launch_fwd<T, DP, 1>(a, st);
+}
+template <typename T> int run_fwd(const AttnArgs& a, int nw, hipStream_t st) {
+  if (a.d <= 32) return launch_fwd_w<T, 32>(a, nw, st);
+  if (a.d <= 64) return launch_fwd_w<T, 64>(a, nw, st);
+  if (a.d <= 96) return launch_fwd_w<T, 96>(a, nw, st);
+  return launch_fwd_w<T, 128>(a, nw, st);
+}
+template <typename T, int DP> int launch_bwd(AttnArgs& a, hipStream_t st) {
+  a.nblk = (a.rows + 127) / 128;
+  if (a.rows) {
+    hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP>), dim3((unsigned)((int64_t)a.b * a.hk * a.nblk)), dim3(256), 0, st, a);
+    MYOLO_CHECK_LAUNCH();
+  }
+  if (a.gk && a.lk) {
+    a.nblk = (a.lk + 127) / 128;
+    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP>), dim3((unsigned)((int64_t)a.b * a.hk * a.nblk)), dim3(256), 0, st, a);
+    MYOLO_CHECK_LAUNCH();
+  }
+  return 0;
+}
+template <typename T> int run_bwd(AttnArgs& a, hipStream_t st) {
+  if (a.d <= 32) return launch_bwd<T, 32>(a, st);
+  if (a.d <= 64) return launch_bwd<T, 64>(a, st);
+  if (a.d <= 96) return launch_bwd<T, 96>(a, st);
+  return launch_bwd<T, 128>(a, st);
+}
+
+}  // namespace
+
+extern "C" int64_t myolo_attn_ws_bytes(const myolo_attn_desc* d, int backward) {
+  if (!desc_ok(d)) return 0;
+  if (backward) return (int64_t)d->b * d->hq * d->lq * 4;
+  const FwdShape f = fwd_shape(d);
+  if (f.nsplit == 1) return 0;
+  return (int64_t)f.nsplit * d->b * d->hq * d->lq * (d->d + 2) * 4;
+}
+
+extern "C" int myolo_attn_fwd(const myolo_attn_desc* d, void* stream) {
+  if (!desc_ok(d) || !(d->scale > 0.f)) return MYOLO_EINVAL;
+  if ((int64_t)d->b * d->lq == 0) return 0;
+  const int es = d->dtype == MYOLO_F16 ? 2 : 4;
+  if (!side_ok(d->q, d->qs, es) || !side_ok(d->o, d->os, es)) return MYOLO_EINVAL;
+  if (d->lk && (!side_ok(d->k, d->ks, es) || !side_ok(d->v, d->vs, es))) return MYOLO_EINVAL;
+  const FwdShape f = fwd_shape(d);
+  AttnArgs a = args_of(d);
+  a.nblk = f.nblk; a.nsplit = f.nsplit; a.part = (float*)d->ws;
+  if ((int64_t)a.b * a.hk * a.nblk * a.nsplit > 0x7fffffff) return MYOLO_EINVAL;
+  if (f.nsplit > 1 && (!d->ws || (uintptr_t)d->ws % 16 || d->ws_bytes < myolo_attn_ws_bytes(d, 0))) return MYOLO_EINVAL;
+  hipStream_t st = (hipStream_t)stream;
+  return d->dtype == MYOLO_F16 ? run_fwd<half_t>(a, f.nw, st) : run_fwd<float>(a, f.nw, st);
+}
+
+extern "C" int myolo_attn_bwd(const myolo_attn_desc* d, void* stream) {
+  if (!desc_ok(d) || !(d->scale > 0.f) || (d->gk == nullptr) != (d->gv == nullptr)) return MYOLO_EINVAL;
+  if (d->b == 0 || (!d->gq && !d->gk)) return 0;
+  const int es = d->dtype == MYOLO_F16 ? 2 : 4;
+  if (d->lq && (!side_ok(d->q, d->qs, es) || !side_ok(d->o, d->os, es) || !side_ok(d->go, d->gos, es) || !d->lse)) return MYOLO_EINVAL;
+  if (d->lk && (!side_ok(d->k, d->ks, es) || !side_ok(d->v, d->vs, es))) return MYOLO_EINVAL;
+  if ((d->gq && d->lq && !side_ok(d->gq, d->gqs, es)) || (d->gk && d->lk && (!side_ok(d->gk, d->gks, es) || !side_ok(d->gv, d->gvs, es))))
+    return MYOLO_EINVAL;
+  if (d->lq && (!d->ws || (uintptr_t)d->ws % 16 || d->ws_bytes < myolo_attn_ws_bytes(d, 1))) return MYOLO_EINVAL;
+  AttnArgs a = args_of(d);
+  if ((int64_t)a.b * a.hk * ((a.rows + 127) / 128) > 0x7fffffff || (int64_t)a.b * a.hk * ((a.lk + 127) / 128) > 0x7fffffff) return MYOLO_EINVAL;
+  a.delta = (float*)d->ws;
+  hipStream_t st = (hipStream_t)stream;
+  return d->dtype == MYOLO_F16 ? run_bwd<half_t>(a, st) : run_bwd<float>(a, st);
+}
