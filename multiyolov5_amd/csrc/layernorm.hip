@@ -4,7 +4,8 @@
 //   gx = rstd * (g - mean g - xhat * mean(g * xhat)),  g = gout * gamma;   dgamma = sum_rows gout * xhat;  dbeta = sum_rows gout
 //
 // The statistics, the row sums and the parameter sums are fp32; the variance is the mean of squared differences from the mean already
-// formed (no E[x^2] - mu^2 cancellation), the result is rounded once.
+// formed (no E[x^2] - mu^2 cancellation), the result is rounded once.  The mean is a true quotient: a constant row whose sum is exact gives
+// xhat = 0 exactly (a product with 1/c, contracted into the subtraction, would leave its rounding times rstd).
 #include "myolo_dev.h"
 
 namespace {
@@ -57,7 +58,7 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void ln_fwd_any_kernel(Rows x, Rows o, int64_t rows, int c, const float* gamma, const float* beta, float eps,
                                                          float* saved) {
   __shared__ float sm[4];
-  const float rc = 1.f / (float)c;
+  const float fc = (float)c;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xp = row_ptr<T>(x, r);
     T* op = row_ptr<T>(o, r);
@@ -67,14 +68,14 @@ __global__ __launch_bounds__(256) void ln_fwd_any_kernel(Rows x, Rows o, int64_t
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s += f[e];
     }
-    const float mu = block_sum<256>(s, sm) * rc;
+    const float mu = block_sum<256>(s, sm) / fc;
     s = 0.f;
     for (int i = threadIdx.x * VEC; i < c; i += 256 * VEC) {
       ldv<T, VEC>(xp + i, f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s += (f[e] - mu) * (f[e] - mu);
     }
-    const float rstd = 1.f / sqrtf(block_sum<256>(s, sm) * rc + eps);
+    const float rstd = 1.f / sqrtf(block_sum<256>(s, sm) / fc + eps);
     if (saved && threadIdx.x == 0) { saved[r] = mu; saved[rows + r] = rstd; }
     for (int i = threadIdx.x * VEC; i < c; i += 256 * VEC) {
       ldv<T, VEC>(xp + i, f);
@@ -89,7 +90,7 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void ln_bwd_any_kernel(Rows go, Rows x, Rows gx, int64_t rows, int c, const float* saved, const float* gamma,
                                                          int acc) {
   __shared__ float sm[4];
-  const float rc = 1.f / (float)c;
+  const float fc = (float)c;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xp = row_ptr<T>(x, r);
     const T* gp = row_ptr<T>(go, r);
@@ -106,8 +107,8 @@ __global__ __launch_bounds__(256) void ln_bwd_any_kernel(Rows go, Rows x, Rows g
         s2 += v * ((f[e] - mu) * rstd);
       }
     }
-    s1 = block_sum<256>(s1, sm) * rc;
-    s2 = block_sum<256>(s2, sm) * rc;
+    s1 = block_sum<256>(s1, sm) / fc;
+    s2 = block_sum<256>(s2, sm) / fc;
     for (int i = threadIdx.x * VEC; i < c; i += 256 * VEC) {
       ldv<T, VEC>(xp + i, f);
       ldv<T, VEC>(gp + i, g);
@@ -119,6 +120,196 @@ __global__ __launch_bounds__(256) void ln_bwd_any_kernel(Rows go, Rows x, Rows g
         for (int e = 0; e < VEC; ++e) f[e] += g[e];
       }
       stv<T, VEC>(op + i, f);
+    }
+  }
+}
+
+// ---- rows held in registers ----------------------------------------------------------------------------------------------------------
+// A row belongs to G adjacent lanes (4 .. 64 of a wave, or the whole workgroup of 256), each holding NV vectors of it: x and gout are read once,
+// their next row is in flight while this one is reduced and written, gamma / beta and the parameter sums stay in registers over all rows
+// of a workgroup.
+template <typename T, int VEC, int NV> struct RowRegs {
+  uint4 raw[VEC > 1 ? NV : 1];
+  T el[VEC > 1 ? 1 : NV];
+  __device__ __forceinline__ void load(const T* p, int t, int g, int c, bool live) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * g + t) * VEC;
+      const bool ok = live && col < c;
+      if constexpr (VEC > 1) raw[i] = ldg16(ok ? (const char*)(p + col) : zero_page());
+      else el[i] = *(const __attribute__((address_space(1))) T*)(ok ? (const char*)(p + col) : zero_page());
+    }
+  }
+  __device__ __forceinline__ void get(int i, float* f) const {
+    if constexpr (VEC > 1) Vec<T>::unpack(raw[i], f);
+    else f[0] = (float)el[i];
+  }
+};
+template <int VEC, int NV> struct ParamRegs {
+  float v[NV * VEC];
+  __device__ __forceinline__ void load(const float* p, int t, int g, int c, float none) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int col = (i * g + t) * VEC + e;
+        v[i * VEC + e] = p ? (col < c ? p[col] : 0.f) : none;
+      }
+  }
+};
+// sum over the G lanes of a row (WIDE: over the workgroup)
+template <bool WIDE> __device__ __forceinline__ float row_sum(float v, int g, float* sm) {
+  if constexpr (WIDE) return block_sum<256>(v, sm);
+  for (int o = g >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+template <typename T, int VEC, int NV, bool WIDE>
+__global__ __launch_bounds__(256) void ln_fwd_kernel(Rows x, Rows o, int64_t rows, int c, int glog, const float* gamma, const float* beta, float eps,
+                                                     float* saved) {
+  __shared__ float sm[4];
+  const int g = WIDE ? 256 : 1 << glog, t = WIDE ? threadIdx.x : threadIdx.x & (g - 1);
+  const int64_t step = WIDE ? gridDim.x : (int64_t)gridDim.x << (8 - glog);
+  int64_t r = WIDE ? blockIdx.x : ((int64_t)blockIdx.x << (8 - glog)) + (threadIdx.x >> glog);
+  const int64_t turns = WIDE ? (rows - blockIdx.x + step - 1) / step : (rows - ((int64_t)blockIdx.x << (8 - glog)) + step - 1) / step;
+  const float fc = (float)c;
+  RowRegs<T, VEC, NV> cur, nxt;
+  cur.load(row_ptr<T>(x, r < rows ? r : 0), t, g, c, r < rows);
+  ParamRegs<VEC, NV> w, b;
+  w.load(gamma, t, g, c, 1.f);
+  b.load(beta, t, g, c, 0.f);
+  for (int64_t it = 0; it < turns; ++it, r += step) {
+    const int64_t rn = r + step;
+    if (it + 1 < turns) nxt.load(row_ptr<T>(x, rn < rows ? rn : 0), t, g, c, rn < rows);
+    float f[NV * VEC], s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      cur.get(i, f + i * VEC);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s += f[i * VEC + e];
+    }
+    const float mu = row_sum<WIDE>(s, g, sm) / fc;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float& v = f[i * VEC + e];
+        v = (i * g + t) * VEC < c ? v - mu : 0.f;
+        s += v * v;
+      }
+    const float rstd = 1.f / sqrtf(row_sum<WIDE>(s, g, sm) / fc + eps);
+    if (r < rows) {
+      if (saved && t == 0) { saved[r] = mu; saved[rows + r] = rstd; }
+      T* op = row_ptr<T>(o, r);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * g + t) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[i * VEC + e] = f[i * VEC + e] * rstd * w.v[i * VEC + e] + b.v[i * VEC + e];
+        if (col < c) stv<T, VEC>(op + col, f + i * VEC);
+      }
+    }
+    cur = nxt;
+  }
+}
+
+// PARAM: the workgroup's sums for gamma / beta go to ws[blockIdx.x][2][c]
+template <typename T, int VEC, int NV, bool WIDE, bool PARAM>
+__global__ __launch_bounds__(256) void ln_bwd_kernel(Rows go, Rows x, Rows gx, int want_gx, int64_t rows, int c, int glog, const float* saved,
+                                                     const float* gamma, int acc, float* ws) {
+  __shared__ float sm[4];
+  extern __shared__ float tot[];                            // PARAM && !WIDE: [2][c]
+  const int g = WIDE ? 256 : 1 << glog, t = WIDE ? threadIdx.x : threadIdx.x & (g - 1);
+  const int64_t step = WIDE ? gridDim.x : (int64_t)gridDim.x << (8 - glog);
+  int64_t r = WIDE ? blockIdx.x : ((int64_t)blockIdx.x << (8 - glog)) + (threadIdx.x >> glog);
+  const int64_t turns = WIDE ? (rows - blockIdx.x + step - 1) / step : (rows - ((int64_t)blockIdx.x << (8 - glog)) + step - 1) / step;
+  const float fc = (float)c;
+  RowRegs<T, VEC, NV> cx, cg, nx, ng;
+  {
+    const int64_t q = r < rows ? r : 0;
+    cx.load(row_ptr<T>(x, q), t, g, c, r < rows);
+    cg.load(row_ptr<T>(go, q), t, g, c, r < rows);
+  }
+  ParamRegs<VEC, NV> w;
+  w.load(gamma, t, g, c, 1.f);
+  float dg[PARAM ? NV * VEC : 1], db[PARAM ? NV * VEC : 1];
+#pragma unroll
+  for (int i = 0; i < (PARAM ? NV * VEC : 1); ++i) dg[i] = db[i] = 0.f;
+  for (int64_t it = 0; it < turns; ++it, r += step) {
+    const int64_t rn = r + step, q = r < rows ? r : 0;
+    const float mu = saved[q], rstd = saved[rows + q];
+    if (it + 1 < turns) {
+      const int64_t qn = rn < rows ? rn : 0;
+      nx.load(row_ptr<T>(x, qn), t, g, c, rn < rows);
+      ng.load(row_ptr<T>(go, qn), t, g, c, rn < rows);
+    }
+    float xh[NV * VEC], v[NV * VEC], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      cx.get(i, xh + i * VEC);
+      cg.get(i, v + i * VEC);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int k = i * VEC + e;
+        xh[k] = r < rows && (i * g + t) * VEC < c ? (xh[k] - mu) * rstd : 0.f;
+        if constexpr (PARAM) { dg[k] += v[k] * xh[k]; db[k] += v[k]; }
+        v[k] *= w.v[k];
+        s1 += v[k];
+        s2 += v[k] * xh[k];
+      }
+    }
+    if (want_gx) {
+      s1 = row_sum<WIDE>(s1, g, sm) / fc;
+      s2 = row_sum<WIDE>(s2, g, sm) / fc;
+      if (r < rows) {
+        T* op = row_ptr<T>(gx, r);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int col = (i * g + t) * VEC;
+          if (col >= c) continue;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[i * VEC + e] = rstd * (v[i * VEC + e] - s1 - xh[i * VEC + e] * s2);
+          if (acc) {
+            float old[VEC];
+            ldv<T, VEC>(op + col, old);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[i * VEC + e] += old[e];
+          }
+          stv<T, VEC>(op + col, v + i * VEC);
+        }
+      }
+    }
+    cx = nx;
+    cg = ng;
+  }
+  if constexpr (PARAM) {
+    float* wp = ws + (int64_t)blockIdx.x * 2 * c;
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < NV * VEC; ++i) {
+        const int col = ((i / VEC) * g + t) * VEC + i % VEC;
+        if (col < c) { wp[col] = dg[i]; wp[c + col] = db[i]; }
+      }
+    } else {
+      // rows of a wave (a butterfly over its groups), then the four waves one after the other: one order, whatever runs when
+      for (int o = g; o < 64; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) { dg[i] += __shfl_xor(dg[i], o, 64); db[i] += __shfl_xor(db[i], o, 64); }
+      for (int k = 0; k < 4; ++k) {
+        if ((threadIdx.x >> 6) == k && (threadIdx.x & 63) < g) {
+#pragma unroll
+          for (int i = 0; i < NV * VEC; ++i) {
+            const int col = ((i / VEC) * g + t) * VEC + i % VEC;
+            if (col < c) {
+              tot[col] = k ? tot[col] + dg[i] : dg[i];
+              tot[c + col] = k ? tot[c + col] + db[i] : db[i];
+            }
+          }
+        }
+        __syncthreads();
+      }
+      for (int i = threadIdx.x; i < 2 * c; i += 256) wp[i] = tot[i];
     }
   }
 }
@@ -145,20 +336,20 @@ __global__ __launch_bounds__(256) void ln_param_any_kernel(Rows go, Rows x, int6
     ws[((int64_t)blockIdx.y * 2 + wv) * c + ch] = (sm[wv][0][lane] + sm[wv][1][lane]) + (sm[wv][2][lane] + sm[wv][3][lane]);
 }
 
-// ws [n][2][c] -> dgamma, dbeta: 16 channels x 16 slices of the partial rows a workgroup, combined in a fixed order
-__global__ __launch_bounds__(256) void ln_param_reduce_kernel(const float* ws, int n, int c, float* dgamma, float* dbeta, int acc) {
-  __shared__ float sm[16][17];
+// ws [n][2][c] -> dgamma, dbeta: 16 channels x 64 slices of the partial rows a workgroup, combined in a fixed order
+__global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* ws, int n, int c, float* dgamma, float* dbeta, int acc) {
+  __shared__ float sm[64][17];
   const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4;
   const int col = blockIdx.x * 16 + cl;                  // 0 .. 2c: gamma's channels, then beta's
   float s = 0.f;
   if (col < 2 * c)
-    for (int i = sl; i < n; i += 16) s += ws[(int64_t)i * 2 * c + col];
+    for (int i = sl; i < n; i += 64) s += ws[(int64_t)i * 2 * c + col];
   sm[sl][cl] = s;
   __syncthreads();
   if (sl == 0 && col < 2 * c) {
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += sm[i][cl];
+    for (int i = 0; i < 64; ++i) s += sm[i][cl];
     float* d = col < c ? dgamma : dbeta;
     if (d) {
       d += col < c ? col : col - c;
@@ -167,7 +358,33 @@ __global__ __launch_bounds__(256) void ln_param_reduce_kernel(const float* ws, i
   }
 }
 
-constexpr int kSlices = 256;
+// how a row is laid out over lanes: vectors a lane, lanes a row (log2), or the whole workgroup; nv == 0: read row by row (any_kernel)
+struct Lay { int nv, glog; bool wide; };
+Lay lay_of(int c, int vec) {
+  const int n = (c + vec - 1) / vec;
+  // the fewest idle lanes of 4 .. 64 times 1 .. 4 vectors, the most lanes where that ties; then whole waves with more, then workgroups; at
+  // most 32 elements a lane (the backward holds seven registers an element: 64 of them spill)
+  Lay best{0, 0, false};
+  int waste = 1 << 30;
+  for (int gl = 6; gl >= 2; --gl)
+    for (int nv = 1; nv <= 4; ++nv)
+      if ((nv << gl) >= n && (nv << gl) - n < waste) { waste = (nv << gl) - n; best = Lay{nv, gl, false}; }
+  if (best.nv) return best;
+  if (vec < 8 && n <= 64 * 8) return Lay{8, 6, false};
+  if (vec == 1 && n <= 64 * 16) return Lay{16, 6, false};
+  for (int nv = 2; nv <= 4; ++nv)
+    if (n <= 256 * nv) return Lay{nv, 8, true};
+  if (vec < 8 && n <= 256 * 8) return Lay{8, 8, true};
+  if (vec == 1 && n <= 256 * 16) return Lay{16, 8, true};
+  return best;
+}
+constexpr int kSlices = 1024;
+// workgroups of the backward (= partial parameter sums): four a CU, each lane group at least four rows
+int bwd_groups(int64_t rows, const Lay& l) {
+  const int64_t per = l.wide ? 1 : 1 << (8 - l.glog);
+  int64_t n = (rows + per * 4 - 1) / (per * 4);
+  return (int)(n < kSlices ? n : kSlices);
+}
 
 bool view_ok(const myolo_tensor& t) {
   return (t.ptr || (int64_t)t.n * t.h * t.w == 0) && (t.dtype == MYOLO_F16 || t.dtype == MYOLO_F32) && t.n >= 0 && t.h >= 0 && t.w >= 0 && t.c >= 1 &&
@@ -182,40 +399,70 @@ bool vec_ok(const myolo_tensor& t) {
   return t.c % seg == 0 && (uintptr_t)t.ptr % 16 == 0 && t.sn % seg == 0 && t.sh % seg == 0 && t.sw % seg == 0;
 }
 
-template <typename T>
+#define LN_BY_NV(CALL)                                                                                                \
+  if (l.wide) {                                                                                                       \
+    if (l.nv == 2) { CALL(2, true); } else if (l.nv == 3) { CALL(3, true); } else if (l.nv == 4) { CALL(4, true); }   \
+    else if (l.nv == 8) { if constexpr (VEC < 8) { CALL(8, true); } }                                                 \
+    else { if constexpr (VEC == 1) { CALL(16, true); } }                                                              \
+  } else if (l.nv == 1) { CALL(1, false); } else if (l.nv == 2) { CALL(2, false); }                                   \
+  else if (l.nv == 3) { CALL(3, false); } else if (l.nv == 4) { CALL(4, false); }                                     \
+  else if (l.nv == 8) { if constexpr (VEC < 8) { CALL(8, false); } }                                                  \
+  else { if constexpr (VEC == 1) { CALL(16, false); } }
+
+template <typename T, int VEC>
 int ln_fwd(const myolo_tensor* x, const float* gamma, const float* beta, float eps, const myolo_tensor* out, float* saved, hipStream_t st) {
   const int64_t rows = (int64_t)x->n * x->h * x->w;
   const Rows rx = rows_of(*x), ro = rows_of(*out);
-  const int grid = (int)(rows < 65536 ? rows : 65536);
-  if (vec_ok(*x) && vec_ok(*out))
-    hipLaunchKernelGGL((ln_fwd_any_kernel<T, ET<T>::SEG>), dim3(grid), dim3(256), 0, st, rx, ro, rows, x->c, gamma, beta, eps, saved);
-  else
-    hipLaunchKernelGGL((ln_fwd_any_kernel<T, 1>), dim3(grid), dim3(256), 0, st, rx, ro, rows, x->c, gamma, beta, eps, saved);
+  const Lay l = lay_of(x->c, VEC);
+  if (!l.nv) {
+    const int grid = (int)(rows < 65536 ? rows : 65536);
+    hipLaunchKernelGGL((ln_fwd_any_kernel<T, VEC>), dim3(grid), dim3(256), 0, st, rx, ro, rows, x->c, gamma, beta, eps, saved);
+  } else {
+    const int64_t per = l.wide ? 1 : 1 << (8 - l.glog), all = (rows + per - 1) / per;
+    const int grid = (int)(all < 2048 ? all : 2048);
+#define LN_FWD(NV, WIDE) \
+  hipLaunchKernelGGL((ln_fwd_kernel<T, VEC, NV, WIDE>), dim3(grid), dim3(256), 0, st, rx, ro, rows, x->c, l.glog, gamma, beta, eps, saved)
+    LN_BY_NV(LN_FWD)
+#undef LN_FWD
+  }
   MYOLO_CHECK_LAUNCH();
   return 0;
 }
 
-template <typename T>
+template <typename T, int VEC>
 int ln_bwd(const myolo_tensor* gout, const myolo_tensor* x, const float* saved, const float* gamma, const myolo_tensor* gx, int acc_x,
            float* dgamma, float* dbeta, int acc_params, float* ws, hipStream_t st) {
   const int64_t rows = (int64_t)x->n * x->h * x->w;
-  const Rows rx = rows_of(*x), rg = rows_of(*gout);
-  if (dgamma || dbeta) {
-    const int ns = (int)(rows < kSlices ? rows : kSlices);
-    if (ns) {
-      hipLaunchKernelGGL((ln_param_any_kernel<T>), dim3((x->c + 63) / 64, ns), dim3(256), 0, st, rg, rx, rows, x->c, saved, ws);
+  const Rows rx = rows_of(*x), rg = rows_of(*gout), ro = gx ? rows_of(*gx) : Rows{};
+  const bool param = dgamma || dbeta;
+  const int c = x->c;
+  const Lay l = lay_of(c, VEC);
+  int ns = 0;
+  if (rows && l.nv) {
+    ns = bwd_groups(rows, l);
+    const int smem = param && !l.wide ? 2 * c * 4 : 0;
+#define LN_BWD(NV, WIDE)                                                                                                                   \
+  if (param) hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, NV, WIDE, true>), dim3(ns), dim3(256), smem, st, rg, rx, ro, gx != nullptr, rows, c, \
+                                l.glog, saved, gamma, acc_x, ws);                                                                          \
+  else hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, NV, WIDE, false>), dim3(ns), dim3(256), 0, st, rg, rx, ro, 1, rows, c, l.glog, saved,     \
+                          gamma, acc_x, ws)
+    if (param || gx) { LN_BY_NV(LN_BWD) }
+#undef LN_BWD
+    MYOLO_CHECK_LAUNCH();
+  } else if (rows) {
+    if (param) {              // (before gx, which may be gout)
+      ns = (int)(rows < 256 ? rows : 256);
+      hipLaunchKernelGGL((ln_param_any_kernel<T>), dim3((c + 63) / 64, ns), dim3(256), 0, st, rg, rx, rows, c, saved, ws);
       MYOLO_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL(ln_param_reduce_kernel, dim3((2 * x->c + 15) / 16), dim3(256), 0, st, ws, ns, x->c, dgamma, dbeta, acc_params);
-    MYOLO_CHECK_LAUNCH();
+    if (gx) {
+      const int grid = (int)(rows < 65536 ? rows : 65536);
+      hipLaunchKernelGGL((ln_bwd_any_kernel<T, VEC>), dim3(grid), dim3(256), 0, st, rg, rx, ro, rows, c, saved, gamma, acc_x);
+      MYOLO_CHECK_LAUNCH();
+    }
   }
-  if (gx && rows) {
-    const Rows ro = rows_of(*gx);
-    const int grid = (int)(rows < 65536 ? rows : 65536);
-    if (vec_ok(*x) && vec_ok(*gout) && vec_ok(*gx))
-      hipLaunchKernelGGL((ln_bwd_any_kernel<T, ET<T>::SEG>), dim3(grid), dim3(256), 0, st, rg, rx, ro, rows, x->c, saved, gamma, acc_x);
-    else
-      hipLaunchKernelGGL((ln_bwd_any_kernel<T, 1>), dim3(grid), dim3(256), 0, st, rg, rx, ro, rows, x->c, saved, gamma, acc_x);
+  if (param) {
+    hipLaunchKernelGGL(ln_param_reduce_kernel, dim3((2 * c + 15) / 16), dim3(1024), 0, st, ws, ns, c, dgamma, dbeta, acc_params);
     MYOLO_CHECK_LAUNCH();
   }
   return 0;
@@ -228,7 +475,10 @@ extern "C" int myolo_layernorm_fwd(const myolo_tensor* x, const float* gamma, co
   if (!x || !out || !view_ok(*x) || !view_ok(*out) || !same_shape(*x, *out) || !(eps >= 0.f)) return MYOLO_EINVAL;
   if ((int64_t)x->n * x->h * x->w == 0) return 0;
   hipStream_t st = (hipStream_t)stream;
-  return x->dtype == MYOLO_F16 ? ln_fwd<half_t>(x, gamma, beta, eps, out, saved, st) : ln_fwd<float>(x, gamma, beta, eps, out, saved, st);
+  const bool v = vec_ok(*x) && vec_ok(*out);
+  if (x->dtype == MYOLO_F16)
+    return v ? ln_fwd<half_t, 8>(x, gamma, beta, eps, out, saved, st) : ln_fwd<half_t, 1>(x, gamma, beta, eps, out, saved, st);
+  return v ? ln_fwd<float, 4>(x, gamma, beta, eps, out, saved, st) : ln_fwd<float, 1>(x, gamma, beta, eps, out, saved, st);
 }
 
 extern "C" int64_t myolo_layernorm_ws_bytes(int64_t rows, int c) {
@@ -246,6 +496,10 @@ extern "C" int myolo_layernorm_bwd(const myolo_tensor* gout, const myolo_tensor*
   if (gx && (!view_ok(*gx) || !same_shape(*x, *gx))) return MYOLO_EINVAL;
   if ((dgamma || dbeta) && rows && (!ws || (uintptr_t)ws % 16 || ws_bytes < myolo_layernorm_ws_bytes(rows, x->c))) return MYOLO_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  return x->dtype == MYOLO_F16 ? ln_bwd<half_t>(gout, x, saved, gamma, gx, acc_x, dgamma, dbeta, acc_params, ws, st)
-                               : ln_bwd<float>(gout, x, saved, gamma, gx, acc_x, dgamma, dbeta, acc_params, ws, st);
+  const bool v = vec_ok(*x) && vec_ok(*gout) && (!gx || vec_ok(*gx));
+  if (x->dtype == MYOLO_F16)
+    return v ? ln_bwd<half_t, 8>(gout, x, saved, gamma, gx, acc_x, dgamma, dbeta, acc_params, ws, st)
+             : ln_bwd<half_t, 1>(gout, x, saved, gamma, gx, acc_x, dgamma, dbeta, acc_params, ws, st);
+  return v ? ln_bwd<float, 4>(gout, x, saved, gamma, gx, acc_x, dgamma, dbeta, acc_params, ws, st)
+           : ln_bwd<float, 1>(gout, x, saved, gamma, gx, acc_x, dgamma, dbeta, acc_params, ws, st);
 }

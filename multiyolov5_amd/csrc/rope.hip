@@ -54,6 +54,100 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a) {
   }
 }
 
+// Vector path: a thread owns one 16-byte unit of pairs of one token (SEG pairs (j, j + npair) in two vectors, or SEG / 2 neighbouring pairs in
+// one) and HC of its heads: the angles are formed once for all of them, behind loads that are already in flight.  Adjacent lanes take
+// adjacent units, then adjacent heads: a wave's accesses are contiguous.  Units behind the pairs copy the pass-through channels.
+template <typename T, bool IL, int HC>
+__global__ __launch_bounds__(256) void rope_vec_kernel(RopeArgs a, int units, int pass, int hl) {
+  constexpr int SEG = ET<T>::SEG, NP = IL ? SEG / 2 : SEG, NV = IL ? 1 : 2;
+  const int per = (units + pass) * hl, heads = a.s[0].h + a.s[1].h;
+  const int64_t total = a.tokens * per;
+  for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < total; w += (int64_t)gridDim.x * 256) {
+    const int64_t tok = w / per, b = tok / a.l, i = tok - b * a.l;
+    const int q = (int)(w - tok * per), h0 = q / (units + pass), un = q - h0 * (units + pass);
+    const int c0 = un < units ? un * SEG : 2 * a.npair + (un - units) * SEG;       // (first channel; the pair's second vector: + npair)
+    uint4 in[HC][NV];
+    char* op[HC];
+#pragma unroll
+    for (int k = 0; k < HC; ++k) {
+      const int h = h0 + k * hl, kh = h - a.s[0].h;
+      const RopeSide& s = kh < 0 ? a.s[0] : a.s[1];
+      const int hh = kh < 0 ? h : kh;
+      const bool ok = h < heads;
+      const char* x = s.x + b * s.sb + i * s.sl + hh * s.sh + c0 * (int)sizeof(T);
+      op[k] = ok ? s.o + b * s.ob + i * s.ol + hh * s.oh + c0 * (int)sizeof(T) : nullptr;
+      in[k][0] = ldg16(ok ? x : zero_page());
+      if constexpr (!IL) in[k][1] = ldg16(ok && un < units ? x + a.npair * (int)sizeof(T) : zero_page());
+    }
+    if (un >= units) {
+#pragma unroll
+      for (int k = 0; k < HC; ++k)
+        if (op[k]) stg16(op[k], in[k][0]);
+      continue;
+    }
+    float sn[NP], cs[NP];
+    const int64_t* pos = a.pos + b * a.pb + i * a.pl;
+#pragma unroll
+    for (int e = 0; e < NP; ++e) turn_of(a, pos, un * NP + e, sn + e, cs + e);
+#pragma unroll
+    for (int k = 0; k < HC; ++k) {
+      if (!op[k]) continue;
+      float u[SEG];
+      Vec<T>::unpack(in[k][0], u);
+      if constexpr (IL) {
+#pragma unroll
+        for (int e = 0; e < NP; ++e) {
+          const float x = u[2 * e], y = u[2 * e + 1];
+          u[2 * e] = x * cs[e] - y * sn[e];
+          u[2 * e + 1] = y * cs[e] + x * sn[e];
+        }
+        stg16(op[k], Vec<T>::pack(u));
+      } else {
+        float v[SEG];
+        Vec<T>::unpack(in[k][1], v);
+#pragma unroll
+        for (int e = 0; e < NP; ++e) {
+          const float x = u[e], y = v[e];
+          u[e] = x * cs[e] - y * sn[e];
+          v[e] = y * cs[e] + x * sn[e];
+        }
+        stg16(op[k], Vec<T>::pack(u));
+        stg16(op[k] + a.npair * (int)sizeof(T), Vec<T>::pack(v));
+      }
+    }
+  }
+}
+
+bool side_vec_ok(const RopeSide& s) {
+  if (!s.h) return true;
+  return !(((uintptr_t)s.x | (uintptr_t)s.o | s.sb | s.sl | s.sh | s.ob | s.ol | s.oh) & 15);
+}
+
+template <typename T> int run_rope(const RopeArgs& a, hipStream_t st) {
+  constexpr int SEG = ET<T>::SEG;
+  const int np = a.interleaved ? SEG / 2 : SEG, heads = a.s[0].h + a.s[1].h;
+  if (!(a.npair % np == 0 && (a.d - 2 * a.npair) % SEG == 0 && side_vec_ok(a.s[0]) && side_vec_ok(a.s[1]))) {
+    const int grid = grid_for(a.tokens * heads * (a.d - a.npair), 256, 1 << 20);
+    hipLaunchKernelGGL(rope_any_kernel<T>, dim3(grid), dim3(256), 0, st, a);
+    MYOLO_CHECK_LAUNCH();
+    return 0;
+  }
+  const int units = a.npair / np, pass = (a.d - 2 * a.npair) / SEG;
+  // four heads a thread where that still leaves four waves for every CU's SIMD, one where the call is that small
+  const int hc = a.tokens * heads * (units + pass) >= 4 * 4 * 256 * 256 ? 4 : 1;
+  const int hl = (heads + hc - 1) / hc;
+  const int grid = grid_for(a.tokens * hl * (units + pass), 256, 1 << 20);
+  if (a.interleaved) {
+    if (hc == 4) hipLaunchKernelGGL((rope_vec_kernel<T, true, 4>), dim3(grid), dim3(256), 0, st, a, units, pass, hl);
+    else hipLaunchKernelGGL((rope_vec_kernel<T, true, 1>), dim3(grid), dim3(256), 0, st, a, units, pass, hl);
+  } else {
+    if (hc == 4) hipLaunchKernelGGL((rope_vec_kernel<T, false, 4>), dim3(grid), dim3(256), 0, st, a, units, pass, hl);
+    else hipLaunchKernelGGL((rope_vec_kernel<T, false, 1>), dim3(grid), dim3(256), 0, st, a, units, pass, hl);
+  }
+  MYOLO_CHECK_LAUNCH();
+  return 0;
+}
+
 }  // namespace
 
 extern "C" int myolo_rope(const myolo_rope_desc* d, void* stream) {
@@ -75,9 +169,5 @@ extern "C" int myolo_rope(const myolo_rope_desc* d, void* stream) {
   a.sign = d->inverse ? -1.f : 1.f;
   for (int j = 0; j < d->npair; ++j) { a.turns[j] = d->turns[j]; a.axis[j] = (unsigned char)d->axis[j]; }
   hipStream_t st = (hipStream_t)stream;
-  const int grid = grid_for(tokens * (d->hq + d->hk) * (d->d - d->npair), 256, 1 << 20);
-  if (d->dtype == MYOLO_F16) hipLaunchKernelGGL(rope_any_kernel<half_t>, dim3(grid), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(rope_any_kernel<float>, dim3(grid), dim3(256), 0, st, a);
-  MYOLO_CHECK_LAUNCH();
-  return 0;
+  return d->dtype == MYOLO_F16 ? run_rope<half_t>(a, st) : run_rope<float>(a, st);
 }
