@@ -22,10 +22,11 @@ struct AttnArgs {
   char *o, *gq, *gk, *gv;
   float *lse, *delta;
   float* part;             // split forward: [split][b*hk][rows][d] unnormalised sums, then [split][b*hk][rows][2] max and denominator
+                           // split dk / dv: [b*hk][nsb][split][dk, dv][128][d] partial sums
   const int *lens, *starts;
   int64_t qs[3], ks[3], vs[3], os[3], gos[3], gqs[3], gks[3], gvs[3];      // bytes
   int b, lq, lk, hq, hk, g, d, causal, window, sinks;
-  int rows, nblk, nsplit;
+  int rows, nblk, nsplit, nsb;        // nsb: key blocks [0, nsb) of the dk / dv pass are split over nsplit workgroups
   float scale, sl2;        // scale, scale * log2(e)
 };
 
@@ -131,22 +132,46 @@ __device__ __forceinline__ float half_sum(float x) {
 }
 
 // ---- what is visible -----------------------------------------------------------------------------------------------------------------
+// Everything here is an interval of integers: masks are one or two unsigned comparisons and a select, never a branch of the lanes.
+struct Range {             // lo <= x < lo + n
+  int lo;
+  unsigned n;
+  __device__ __forceinline__ bool has(int x) const { return (unsigned)x - (unsigned)lo < n; }
+};
+__device__ __forceinline__ Range range_of(int lo, int hi) { return Range{lo, hi > lo ? (unsigned)hi - (unsigned)lo : 0u}; }
+struct Keys {              // keys [0, first) and the band
+  int first;
+  Range band;
+  __device__ __forceinline__ bool has(int j) const { return band.has(j) | (j < first); }
+};
 struct Vis {
   int start, len, causal, window, sinks;
-  __device__ __forceinline__ bool sees(int p, int j) const {
-    const int dist = p > j ? p - j : j - p;
-    return j < len && (!causal || j <= p) && (!window || dist < window || j < sinks);
+  // the keys that some query of the consecutive positions [p0, p1] sees
+  __device__ __forceinline__ Keys keys(int p0, int p1) const {
+    const int hi = causal ? min(len, p1 + 1) : len;
+    return Keys{window ? min(sinks, hi) : 0, window ? range_of(max(0, p0 - window + 1), min(hi, p1 + window)) : range_of(0, hi)};
+  }
+  // the positions that see key j
+  __device__ __forceinline__ Range queries(int j) const {
+    const bool band = window && j >= sinks;
+    int lo = band ? j - window + 1 : -(1 << 30);
+    if (causal) lo = max(lo, j);
+    return range_of(lo, j < len ? (band ? j + window : 1 << 30) : lo);
+  }
+  // the positions that see some key
+  __device__ __forceinline__ Range rows() const {
+    const bool band = window && !sinks;
+    const int lo = causal ? 0 : band ? 1 - window : -(1 << 30);
+    return range_of(lo, len > 0 ? (band ? len + window - 1 : 1 << 30) : lo);
   }
   // every query of positions [p0, p1] sees every key of [j0, j1]
   __device__ __forceinline__ bool all(int p0, int p1, int j0, int j1) const {
-    return j1 < len && (!causal || j1 <= p0) && (!window || (p1 - j0 < window && j1 - p0 < window) || j1 < sinks);
+    return (j1 < len) & (!causal | (j1 <= p0)) & (!window | ((p1 - j0 < window) & (j1 - p0 < window)) | (j1 < sinks));
   }
   // some query of [p0, p1] may see some key of [j0, j1]
   __device__ __forceinline__ bool any(int p0, int p1, int j0, int j1) const {
-    return j0 < len && (!causal || j0 <= p1) && (!window || (p0 - j1 < window && j0 - p1 < window) || j0 < sinks);
+    return (j0 < len) & (!causal | (j0 <= p1)) & (!window | ((p0 - j1 < window) & (j0 - p1 < window)) | (j0 < sinks));
   }
-  // some query of [p0, p1] sees key j (exact: positions are consecutive)
-  __device__ __forceinline__ bool key(int p0, int p1, int j) const { return j >= 0 && any(p0, p1, j, j); }
 };
 // (start is clamped to where nothing changes any more, so that positions and distances stay within 32 bits: all lengths <= 2^28)
 __device__ __forceinline__ Vis vis_of(const AttnArgs& a, int b) {
@@ -178,7 +203,7 @@ template <typename T, int DP, int ROWS, int NT> struct Stage {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int u = tid + i * NT, r = u / CH, c = u - r * CH;
-      const bool ok = u < N && c * EC < d && row_ok(r);
+      const bool ok = (u < N) & (c * EC < d) & row_ok(r);
       v[i] = ldg16(ok ? base + (int64_t)r * stride + c * 16 : zero_page());
     }
   }
@@ -201,11 +226,11 @@ __device__ __forceinline__ int xcd_order(int id, int n) {
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
   constexpr int BK = sizeof(T) == 2 || NW > 1 ? 64 : 32, U = BK / 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
   using TL = Tile<T, DL>;
   __shared__ uint4 sK[BK * TL::CH], sV[BK * TL::CH];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int sp = SPLIT ? id % a.nsplit : 0;
   if (SPLIT) id /= a.nsplit;
@@ -224,7 +249,7 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
   Frag<T> qf[KS];
   const char* qp = a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
 #pragma unroll
-  for (int s = 0; s < KS; ++s) frag_global(qf[s], qp + (s * 16 + h * 8) * sizeof(T), live && s * 16 + h * 8 < a.d);
+  for (int s = 0; s < KS; ++s) frag_global(qf[s], qp + (s * 16 + h * 8) * sizeof(T), live & (s * 16 + h * 8 < a.d));
 
   const char* kp = a.k + b * a.ks[0] + kh * a.ks[2];
   const char* vp = a.v + b * a.vs[0] + kh * a.vs[2];
@@ -234,24 +259,29 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
   float mx = -INFINITY, l = 0.f;
 
   const TileList tl = tiles_of(vis, pb0, pb1, BK);
+  const Keys bkeys = vis.keys(pb0, pb1), lkeys = vis.keys(p, p);       // the workgroup's keys, the lane's
   int t0 = 0, t1 = tl.n;
   if (SPLIT) {
     const int per = (tl.n + a.nsplit - 1) / a.nsplit;
     t0 = min(sp * per, tl.n);
     t1 = min(t0 + per, tl.n);
   }
+  // the next tile's global loads are in flight while this one is computed
+  Stage<T, DP, BK, NT> gk, gv;
+  auto fetch = [&](int t) {
+    const int j0 = tl.at(t) * BK;
+    auto ok = [&](int r) { return bkeys.has(j0 + r); };
+    gk.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.d, tid, ok);
+    gv.load(vp + (int64_t)j0 * a.vs[1], a.vs[1], a.d, tid, ok);
+  };
+  if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     const int j0 = tl.at(t) * BK;
-    {
-      Stage<T, DP, BK, NT> gk, gv;
-      auto ok = [&](int r) { return vis.key(pb0, pb1, j0 + r); };
-      gk.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.d, tid, ok);
-      gv.load(vp + (int64_t)j0 * a.vs[1], a.vs[1], a.d, tid, ok);
-      __syncthreads();
-      gk.template store<DL>(sK, tid);
-      gv.template store<DL>(sV, tid);
-      __syncthreads();
-    }
+    if (t > t0) __syncthreads();
+    gk.template store<DL>(sK, tid);
+    gv.template store<DL>(sV, tid);
+    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
     if (!vis.any(pw0, pw1, j0, j0 + BK - 1)) continue;
     f16_t s[U];
 #pragma unroll
@@ -269,7 +299,7 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (!vis.sees(p, j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h)) s[u][r] = -INFINITY;
+          s[u][r] = lkeys.has(j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[u][r] : -INFINITY;
     }
     float m2 = s[0][0];
 #pragma unroll
@@ -384,11 +414,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 constexpr float kPShift = 12.f, kPUnshift = 1.f / 4096.f;
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_bwd_q_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
   constexpr int NW = 4, BK = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
   using TL = Tile<T, DL>;
   __shared__ uint4 sK[BK * TL::CH], sV[BK * TL::CH];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int id = xcd_order(blockIdx.x, gridDim.x);
   const int blk = a.nblk - 1 - id % a.nblk, bh = id / a.nblk;
   const int b = bh / a.hk, kh = bh - b * a.hk;
@@ -410,7 +440,7 @@ __global__ __launch_bounds__(256) void attn_bwd_q_kernel(AttnArgs a) {
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     const int c = (s * 16 + h * 8);
-    const bool ok = live && c < a.d;
+    const bool ok = live & (c < a.d);
     Frag<T> of;
     frag_global(qf[s], qp + c * sizeof(T), ok);
     frag_global(gf[s], gp + c * sizeof(T), ok);
@@ -428,18 +458,23 @@ __global__ __launch_bounds__(256) void attn_bwd_q_kernel(AttnArgs a) {
   for (int m = 0; m < MT; ++m) dq[m] = f16_t{};
 
   const TileList tl = tiles_of(vis, pb0, pb1, BK);
-  for (int t = 0; a.gq && t < tl.n; ++t) {
+  const Keys bkeys = vis.keys(pb0, pb1), lkeys = vis.keys(p, p);       // the workgroup's keys, the lane's
+  const int nt = a.gq ? tl.n : 0;
+  Stage<T, DP, BK, NT> gk, gv;
+  auto fetch = [&](int t) {
     const int j0 = tl.at(t) * BK;
-    {
-      Stage<T, DP, BK, NT> gk, gv;
-      auto ok = [&](int r) { return vis.key(pb0, pb1, j0 + r); };
-      gk.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.d, tid, ok);
-      gv.load(vp + (int64_t)j0 * a.vs[1], a.vs[1], a.d, tid, ok);
-      __syncthreads();
-      gk.template store<DL>(sK, tid);
-      gv.template store<DL>(sV, tid);
-      __syncthreads();
-    }
+    auto ok = [&](int r) { return bkeys.has(j0 + r); };
+    gk.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.d, tid, ok);
+    gv.load(vp + (int64_t)j0 * a.vs[1], a.vs[1], a.d, tid, ok);
+  };
+  if (nt) fetch(0);
+  for (int t = 0; t < nt; ++t) {
+    const int j0 = tl.at(t) * BK;
+    if (t) __syncthreads();
+    gk.template store<DL>(sK, tid);
+    gv.template store<DL>(sV, tid);
+    __syncthreads();
+    if (t + 1 < nt) fetch(t + 1);
     if (!vis.any(pw0, pw1, j0, j0 + BK - 1)) continue;
     const bool all = vis.all(pw0, pw1, j0, j0 + BK - 1);
 #pragma unroll
@@ -454,9 +489,10 @@ __global__ __launch_bounds__(256) void attn_bwd_q_kernel(AttnArgs a) {
         dp = mma(f, gf[k], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, -lse)) * (dp[r] - delta);
-        s[r] = all || vis.sees(p, j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? x : 0.f;
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, -lse)) * (dp[r] - delta);
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = lkeys.has(j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[r] : 0.f;
       }
       Frag<T> d0, d1, kf;
       frag_from<0>(d0, s);
@@ -482,23 +518,45 @@ __global__ __launch_bounds__(256) void attn_bwd_q_kernel(AttnArgs a) {
 }
 
 // ---- backward: dk, dv ----------------------------------------------------------------------------------------------------------------
-// a wave owns 32 keys (operands and both accumulators in registers), the workgroup's four waves walk the queries that may see its 128 keys
-// and, for each, the heads of the group: the gradient of a shared head is one sum in one place
+// A wave owns 32 keys (operands and both accumulators in registers); the workgroup's four waves walk the query tiles that may see its 128
+// keys, once for every head of the group: the gradient of a shared head is one sum in one place.  Blocks that hold sinks see every query,
+// and few blocks leave CUs idle: blocks [0, nsb) share their walk between nsplit workgroups, whose partial sums a second kernel adds in
+// a fixed order.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_bwd_kv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
   constexpr int NW = 4, BQ = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
   using TL = Tile<T, DL>;
   __shared__ uint4 sQ[BQ * TL::CH], sG[BQ * TL::CH];
   __shared__ float sL[BQ], sD[BQ];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
-  const int id = xcd_order(blockIdx.x, gridDim.x);
-  const int blk = id % a.nblk, bh = id / a.nblk;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int per = a.nblk + a.nsb * (a.nsplit - 1);            // workgroups a (batch, key head)
+  const int id = xcd_order(blockIdx.x, gridDim.x), bh = id / per, it = id - bh * per;
+  const bool part = it < a.nsb * a.nsplit && a.nsplit > 1;
+  const int blk = part ? it / a.nsplit : it - a.nsb * (a.nsplit - 1), sp = part ? it - blk * a.nsplit : 0;
   const int b = bh / a.hk, kh = bh - b * a.hk;
   const Vis vis = vis_of(a, b);
   const int k0 = blk * 32 * NW, k1 = min(k0 + 32 * NW, a.lk) - 1;
   const int kw0 = k0 + wv * 32, kw1 = min(kw0 + 31, a.lk - 1);
   const int key = kw0 + (lane & 31);
-  const bool live = key < a.lk, seen = key < vis.len;
+  const bool seen = key < vis.len;
+  const Range rows = vis.rows();
+  Range lrows = vis.queries(key);                            // the lane's queries; none behind the last one
+  lrows.n = min(lrows.n, (unsigned)max(vis.start + a.lq - lrows.lo, 0));
+
+  // queries that may see a key of [k0, k1]
+  int ilo = 0, ihi = k0 < vis.len ? a.lq - 1 : -1;
+  if (vis.causal) ilo = max(ilo, k0 - vis.start);
+  if (vis.window && k0 >= vis.sinks) {
+    ihi = min(ihi, k1 + vis.window - 1 - vis.start);
+    ilo = max(ilo, k0 - vis.window + 1 - vis.start);
+  }
+  const int q0 = ilo / BQ, nq = ihi >= ilo ? ihi / BQ - q0 + 1 : 0;
+  int t0 = 0, t1 = nq * a.g;
+  if (part) {
+    const int n = (t1 + a.nsplit - 1) / a.nsplit;
+    t0 = min(sp * n, t1);
+    t1 = min(t0 + n, t1);
+  }
 
   Frag<T> kf[KS], vf[KS];
   const char* kp = a.k + b * a.ks[0] + kh * a.ks[2] + (int64_t)key * a.ks[1];
@@ -506,93 +564,106 @@ __global__ __launch_bounds__(256) void attn_bwd_kv_kernel(AttnArgs a) {
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     const int c = s * 16 + h * 8;
-    frag_global(kf[s], kp + c * sizeof(T), seen && c < a.d);
-    frag_global(vf[s], vp + c * sizeof(T), seen && c < a.d);
+    frag_global(kf[s], kp + c * sizeof(T), seen & (c < a.d));
+    frag_global(vf[s], vp + c * sizeof(T), seen & (c < a.d));
   }
   f16_t dk[MT], dv[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) dk[m] = dv[m] = f16_t{};
 
-  // queries that may see a key of [k0, k1]: positions [plo, phi]
-  int ilo = 0, ihi = a.lq - 1;
-  if (k0 >= vis.len) ihi = -1;
-  if (vis.causal) ilo = max(ilo, k0 - vis.start);
-  if (vis.window && k0 >= vis.sinks) {
-    ihi = min(ihi, k1 + vis.window - 1 - vis.start);
-    ilo = max(ilo, k0 - vis.window + 1 - vis.start);
-  }
-  for (int hd = 0; hd < a.g; ++hd) {
-    const int head = kh * a.g + hd;
-    const char* qp = a.q + b * a.qs[0] + head * a.qs[2];
-    const char* gp = a.go + b * a.gos[0] + head * a.gos[2];
-    const int64_t lrow = ((int64_t)b * a.hq + head) * a.lq;
-    for (int i0 = ilo / BQ * BQ; i0 <= ihi; i0 += BQ) {
-      {
-        // rows behind the last query and rows that see nothing (lse = -inf) enter as zeros
-        Stage<T, DP, BQ, NT> gq, gg;
-        auto ok = [&](int r) { return i0 + r < a.lq && a.lse[lrow + i0 + r] != -INFINITY; };
-        gq.load(qp + (int64_t)i0 * a.qs[1], a.qs[1], a.d, tid, ok);
-        gg.load(gp + (int64_t)i0 * a.gos[1], a.gos[1], a.d, tid, ok);
-        float ls = -INFINITY, de = 0.f;
-        if (tid < BQ && i0 + tid < a.lq) {
-          ls = a.lse[lrow + i0 + tid];
-          de = a.delta[lrow + i0 + tid];
-        }
-        __syncthreads();
-        gq.template store<DL>(sQ, tid);
-        gg.template store<DL>(sG, tid);
-        if (tid < BQ) {
-          sL[tid] = kPShift - ls;
-          sD[tid] = ls == -INFINITY ? 0.f : de * kPUnshift;
-        }
-        __syncthreads();
+  Stage<T, DP, BQ, NT> gq, gg;
+  float nl = 0.f, nd = 0.f;
+  auto fetch = [&](int t) {
+    const int hd = t / nq, i0 = (q0 + t - hd * nq) * BQ, head = kh * a.g + hd;
+    // rows behind the last query and rows that see nothing enter as zeros, whatever they hold
+    auto ok = [&](int r) { return (i0 + r < a.lq) & rows.has(vis.start + i0 + r); };
+    gq.load(a.q + b * a.qs[0] + head * a.qs[2] + (int64_t)i0 * a.qs[1], a.qs[1], a.d, tid, ok);
+    gg.load(a.go + b * a.gos[0] + head * a.gos[2] + (int64_t)i0 * a.gos[1], a.gos[1], a.d, tid, ok);
+    if (tid < BQ) {
+      const bool on = ok(tid);
+      const int64_t lr = ((int64_t)b * a.hq + head) * a.lq + (on ? i0 + tid : 0);
+      nl = on ? kPShift - a.lse[lr] : 0.f;
+      nd = on ? a.delta[lr] * kPUnshift : 0.f;
+    }
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
+    const int hd = t / nq, i0 = (q0 + t - hd * nq) * BQ;
+    if (t > t0) __syncthreads();
+    gq.template store<DL>(sQ, tid);
+    gg.template store<DL>(sG, tid);
+    if (tid < BQ) { sL[tid] = nl; sD[tid] = nd; }
+    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
+    const int p0 = vis.start + i0, p1 = p0 + BQ - 1;
+    if (kw0 > kw1 || !vis.any(p0, p1, kw0, kw1)) continue;
+    const bool all = kw0 + 31 < a.lk && i0 + BQ <= a.lq && vis.all(p0, p1, kw0, kw1);
+#pragma unroll 1
+    for (int u = 0; u < BQ / 32; ++u) {
+      f16_t s = f16_t{}, dp = f16_t{};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        Frag<T> f;
+        TL::row_frag(f, sQ, u * 32 + (lane & 31), k * 2 + h);
+        s = mma(f, kf[k], s);
+        TL::row_frag(f, sG, u * 32 + (lane & 31), k * 2 + h);
+        dp = mma(f, vf[k], dp);
       }
-      const int p0 = vis.start + i0, p1 = p0 + BQ - 1;
-      if (kw0 > kw1 || !vis.any(p0, p1, kw0, kw1)) continue;
-      const bool all = kw0 + 31 < a.lk && i0 + BQ <= a.lq && vis.all(p0, p1, kw0, kw1);
 #pragma unroll
-      for (int u = 0; u < BQ / 32; ++u) {
-        f16_t s = f16_t{}, dp = f16_t{};
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int qb = u * 32 + 8 * r4 + 4 * h;
+        const f4_t l4 = *reinterpret_cast<const f4_t*>(sL + qb), d4 = *reinterpret_cast<const f4_t*>(sD + qb);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          Frag<T> f;
-          TL::row_frag(f, sQ, u * 32 + (lane & 31), k * 2 + h);
-          s = mma(f, kf[k], s);
-          TL::row_frag(f, sG, u * 32 + (lane & 31), k * 2 + h);
-          dp = mma(f, vf[k], dp);
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * r4 + e;
+          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, l4[e]));
+          dp[r] = s[r] * fmaf(dp[r], kPUnshift, -d4[e]);
         }
+      }
+      if (!all) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int q = u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, sL[q]));
-          const bool on = all || (i0 + q < a.lq && sL[q] != INFINITY && live && vis.sees(p0 + q, key));
-          s[r] = on ? x : 0.f;
-          dp[r] = on ? x * fmaf(dp[r], kPUnshift, -sD[q]) : 0.f;
+          const bool on = lrows.has(p0 + q);
+          s[r] = on ? s[r] : 0.f;
+          dp[r] = on ? dp[r] : 0.f;
         }
-        Frag<T> f0, f1, c;
-        frag_from<0>(f0, s);
-        frag_from<1>(f1, s);
+      }
+      Frag<T> f0, f1, c;
+      frag_from<0>(f0, s);
+      frag_from<1>(f1, s);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          TL::col_frag(c, sG, u * 32, m * 32, lane);
-          dv[m] = mma(f0, c, dv[m]);
-          TL::col_frag(c, sG, u * 32 + 16, m * 32, lane);
-          dv[m] = mma(f1, c, dv[m]);
-        }
-        frag_from<0>(f0, dp);
-        frag_from<1>(f1, dp);
+      for (int m = 0; m < MT; ++m) {
+        TL::col_frag(c, sG, u * 32, m * 32, lane);
+        dv[m] = mma(f0, c, dv[m]);
+        TL::col_frag(c, sG, u * 32 + 16, m * 32, lane);
+        dv[m] = mma(f1, c, dv[m]);
+      }
+      frag_from<0>(f0, dp);
+      frag_from<1>(f1, dp);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          TL::col_frag(c, sQ, u * 32, m * 32, lane);
-          dk[m] = mma(f0, c, dk[m]);
-          TL::col_frag(c, sQ, u * 32 + 16, m * 32, lane);
-          dk[m] = mma(f1, c, dk[m]);
-        }
+      for (int m = 0; m < MT; ++m) {
+        TL::col_frag(c, sQ, u * 32, m * 32, lane);
+        dk[m] = mma(f0, c, dk[m]);
+        TL::col_frag(c, sQ, u * 32 + 16, m * 32, lane);
+        dk[m] = mma(f1, c, dk[m]);
       }
     }
   }
   // accumulators: column (lane % 32) = channel, rows = keys
   const int col = lane & 31;
+  if (part) {
+    float* pk = a.part + (((int64_t)bh * a.nsb + blk) * a.nsplit + sp) * (2 * 32 * NW) * a.d;
+    float* pv = pk + 32 * NW * a.d;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int o = (wv * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) * a.d + m * 32 + col;
+        if (m * 32 + col < a.d) { pk[o] = dk[m][r]; pv[o] = dv[m][r]; }
+      }
+    return;
+  }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -603,6 +674,26 @@ __global__ __launch_bounds__(256) void attn_bwd_kv_kernel(AttnArgs a) {
         reinterpret_cast<T*>(a.gv + b * a.gvs[0] + kh * a.gvs[2] + (int64_t)kk * a.gvs[1])[m * 32 + col] = (T)(dv[m][r] * kPUnshift);
       }
     }
+}
+
+// adds the partial sums of the split key blocks
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bwd_kv_join_kernel(AttnArgs a) {
+  const int c4 = a.d / 4, per = 2 * 128 * c4;
+  const int64_t total = (int64_t)a.b * a.hk * a.nsb * per;
+  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
+    const int64_t bb = v / per;
+    const int q = (int)(v - bb * per), which = q / (128 * c4), o = q - which * 128 * c4, kr = o / c4, c = (o - kr * c4) * 4;
+    const int bh = (int)(bb / a.nsb), kk = (int)(bb - (int64_t)bh * a.nsb) * 128 + kr, b = bh / a.hk, kh = bh - b * a.hk;
+    if (kk >= a.lk) continue;
+    const float* p = a.part + bb * a.nsplit * 2 * 128 * a.d + (int64_t)which * 128 * a.d + kr * a.d + c;
+    f4_t s = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < a.nsplit; ++i) s += *reinterpret_cast<const f4_t*>(p + (int64_t)i * 2 * 128 * a.d);
+    const float f = which ? kPUnshift : a.scale;
+    T* g = which ? (T*)(a.gv + b * a.gvs[0] + kh * a.gvs[2] + (int64_t)kk * a.gvs[1]) : (T*)(a.gk + b * a.gks[0] + kh * a.gks[2] + (int64_t)kk * a.gks[1]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) g[c + e] = (T)(s[e] * f);
+  }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
@@ -637,6 +728,32 @@ FwdShape fwd_shape(const myolo_attn_desc* d) {
   f.nsplit = n < 2 ? 1 : (int)n;
   return f;
 }
+struct KvShape { int nblk, nsb, nsplit; };
+KvShape kv_shape(const myolo_attn_desc* d) {
+  const int bq = d->dtype == MYOLO_F16 ? 64 : 32;
+  const int64_t g = d->hq / d->hk, bh = (int64_t)d->b * d->hk;
+  KvShape k{(d->lk + 127) / 128, 0, 1};
+  const int64_t full = (d->lq + bq - 1) / bq * g, total = bh * k.nblk;
+  if (!total || !full) return k;
+  int64_t n = 1;
+  if (d->window && d->sinks) {          // a block of sinks walks every query, its neighbours the band: cut it to their length
+    const int64_t band = (((int64_t)d->window * (d->causal ? 1 : 2) + 127) / bq + 2) * g;
+    n = (full + band - 1) / band;
+    if (n > 1) k.nsb = (int)(((d->sinks < d->lk ? d->sinks : d->lk) + 127) / 128);
+  }
+  if (total < 512) {                    // fewer than two workgroups a CU: every block is shared
+    k.nsb = k.nblk;
+    const int64_t w = (512 + total - 1) / total;
+    if (w > n) n = w;
+  }
+  if (n > full) n = full;
+  if (n > 32) n = 32;
+  while (n > 1 && bh * k.nsb * n * 256 * d->d * 4 > (256ll << 20)) --n;      // scratch stays under 256 MiB
+  k.nsplit = (int)n;
+  if (n == 1) k.nsb = 0;
+  return k;
+}
+int64_t delta_bytes(const myolo_attn_desc* d) { return ((int64_t)d->b * d->hq * d->lq * 4 + 15) / 16 * 16; }
 void bytes3(int64_t* o, const int64_t* s, int64_t es) { for (int i = 0; i < 3; ++i) o[i] = s[i] * es; }
 AttnArgs args_of(const myolo_attn_desc* d) {
   const int64_t es = d->dtype == MYOLO_F16 ? 2 : 4;
@@ -676,31 +793,39 @@ template <typename T> int run_fwd(const AttnArgs& a, int nw, hipStream_t st) {
   if (a.d <= 96) return launch_fwd_w<T, 96>(a, nw, st);
   return launch_fwd_w<T, 128>(a, nw, st);
 }
-template <typename T, int DP> int launch_bwd(AttnArgs& a, hipStream_t st) {
+template <typename T, int DP> int launch_bwd(AttnArgs& a, const KvShape& kv, hipStream_t st) {
   a.nblk = (a.rows + 127) / 128;
   if (a.rows) {
     hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP>), dim3((unsigned)((int64_t)a.b * a.hk * a.nblk)), dim3(256), 0, st, a);
     MYOLO_CHECK_LAUNCH();
   }
   if (a.gk && a.lk) {
-    a.nblk = (a.lk + 127) / 128;
-    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP>), dim3((unsigned)((int64_t)a.b * a.hk * a.nblk)), dim3(256), 0, st, a);
+    const int64_t bh = (int64_t)a.b * a.hk;
+    a.nblk = kv.nblk; a.nsb = kv.nsb; a.nsplit = kv.nsplit;
+    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP>), dim3((unsigned)(bh * (kv.nblk + kv.nsb * (kv.nsplit - 1)))), dim3(256), 0, st, a);
     MYOLO_CHECK_LAUNCH();
+    if (kv.nsplit > 1) {
+      hipLaunchKernelGGL((attn_bwd_kv_join_kernel<T>), dim3(grid_for(bh * kv.nsb * 2 * 128 * (a.d / 4), 256, 4096)), dim3(256), 0, st, a);
+      MYOLO_CHECK_LAUNCH();
+    }
   }
   return 0;
 }
-template <typename T> int run_bwd(AttnArgs& a, hipStream_t st) {
-  if (a.d <= 32) return launch_bwd<T, 32>(a, st);
-  if (a.d <= 64) return launch_bwd<T, 64>(a, st);
-  if (a.d <= 96) return launch_bwd<T, 96>(a, st);
-  return launch_bwd<T, 128>(a, st);
+template <typename T> int run_bwd(AttnArgs& a, const KvShape& kv, hipStream_t st) {
+  if (a.d <= 32) return launch_bwd<T, 32>(a, kv, st);
+  if (a.d <= 64) return launch_bwd<T, 64>(a, kv, st);
+  if (a.d <= 96) return launch_bwd<T, 96>(a, kv, st);
+  return launch_bwd<T, 128>(a, kv, st);
 }
 
 }  // namespace
 
 extern "C" int64_t myolo_attn_ws_bytes(const myolo_attn_desc* d, int backward) {
   if (!desc_ok(d)) return 0;
-  if (backward) return (int64_t)d->b * d->hq * d->lq * 4;
+  if (backward) {
+    const KvShape k = kv_shape(d);
+    return delta_bytes(d) + (k.nsplit > 1 ? (int64_t)d->b * d->hk * k.nsb * k.nsplit * 256 * d->d * 4 : 0);
+  }
   const FwdShape f = fwd_shape(d);
   if (f.nsplit == 1) return 0;
   return (int64_t)f.nsplit * d->b * d->hq * d->lq * (d->d + 2) * 4;
@@ -731,8 +856,10 @@ extern "C" int myolo_attn_bwd(const myolo_attn_desc* d, void* stream) {
     return MYOLO_EINVAL;
   if (d->lq && (!d->ws || (uintptr_t)d->ws % 16 || d->ws_bytes < myolo_attn_ws_bytes(d, 1))) return MYOLO_EINVAL;
   AttnArgs a = args_of(d);
-  if ((int64_t)a.b * a.hk * ((a.rows + 127) / 128) > 0x7fffffff || (int64_t)a.b * a.hk * ((a.lk + 127) / 128) > 0x7fffffff) return MYOLO_EINVAL;
+  const KvShape kv = kv_shape(d);
+  if ((int64_t)a.b * a.hk * ((a.rows + 127) / 128) > 0x7fffffff || (int64_t)a.b * a.hk * (kv.nblk + (int64_t)kv.nsb * kv.nsplit) > 0x7fffffff) return MYOLO_EINVAL;
   a.delta = (float*)d->ws;
+  a.part = (float*)((char*)d->ws + delta_bytes(d));
   hipStream_t st = (hipStream_t)stream;
-  return d->dtype == MYOLO_F16 ? run_bwd<half_t>(a, st) : run_bwd<float>(a, st);
+  return d->dtype == MYOLO_F16 ? run_bwd<half_t>(a, kv, st) : run_bwd<float>(a, kv, st);
 }
