@@ -6,7 +6,6 @@ The arithmetic is in libmyolo (csrc/layernorm.hip, csrc/rope.hip, csrc/attention
 tensors' device, allocates its results and scratch with torch's allocator and never synchronises, so all of them can be captured into a
 graph.  There is no CPU path.
 """
-import contextlib
 import ctypes as C
 import functools
 import math
@@ -17,6 +16,10 @@ from .. import _lib as L
 
 ATTN_MAX_DIM = 128
 _P3 = C.c_int64 * 3
+_stream = torch._C._cuda_getCurrentRawStream          # (device index) -> the current stream's handle
+# A call's checks and descriptor depend on sizes, strides, types and options alone: they are worked out once per signature (the host's time is
+# what bounds small calls), then the addresses are filled in.
+_signature = functools.lru_cache(maxsize=1024)
 
 
 def _tensor(t, what, dtype=None, dim=None):
@@ -31,41 +34,42 @@ def _tensor(t, what, dtype=None, dim=None):
         raise L.MyoloError(f'{what} must have {dim} dimensions, got {tuple(t.shape)}')
 
 
-def _same_device(t, *others):
+def _device(t, *others):
+    """the tensors' common device index"""
+    dev = t.get_device()
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != dev:
             raise L.MyoloError(f'tensors on {t.device} and {o.device} in one call')
+    return dev
 
 
-def _on(t):
-    """launches go to the tensors' device (and its current stream), whatever the current device is"""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _launch(dev, name, *args):
+    """a library call on `dev` and its current stream, whatever the current device is"""
+    fn = getattr(L.lib(), name)
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        L.check(rc, name)
+
+
+def _needs_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _first_order(fn):
+    """backward(ctx, *grads) that refuses to be differentiated again; the check costs nothing where no graph is recorded"""
+    once = torch.autograd.function.once_differentiable(fn)
+    return staticmethod(lambda ctx, *g: once(ctx, *g) if torch.is_grad_enabled() else fn(ctx, *g))
 
 
 # ---- layer norm ------------------------------------------------------------------------------------------------------------------------
-def _rows(x):
-    """(tensor whose memory the view describes, L.Tensor of its rows): last dimension = channels, the others numbered in order.  A view whose
-    leading dimensions do not reduce to three strides, or whose channels are not adjacent, is copied."""
-    if x.dim() == 0:
-        raise L.MyoloError('layer_norm: a tensor with a channel dimension is needed')
-    c = x.shape[-1]
-    if c < 1 or c >= 1 << 31:
-        raise L.MyoloError(f'layer_norm: {c} channels')
-    if x.stride(-1) != 1 and c > 1:
-        x = x.contiguous()
-    n, s = _lead(x)
-    if n is None:
-        x = x.contiguous()
-        n, s = _lead(x)
-    if n is None:
-        raise L.MyoloError('layer_norm: more than 2^31 - 1 rows in one dimension')
-    return x, L.Tensor(x.data_ptr(), n[0], n[1], n[2], c, s[0], s[1], s[2], L.DT[x.dtype], 0)
-
-
-def _lead(x):
-    """leading dimensions merged where their strides allow, padded to three: (sizes, strides), or (None, None)"""
+def _lead(shape, stride):
+    """leading dimensions merged where their strides allow, padded to three: sizes + strides, or None"""
     sizes, strides = [], []
-    for n, s in zip(x.shape[:-1], x.stride()[:-1]):
+    for n, s in zip(shape[:-1], stride[:-1]):
         if n == 1:
             continue
         if sizes and strides[-1] == n * s and sizes[-1] * n < 1 << 31:
@@ -74,85 +78,126 @@ def _lead(x):
             sizes.append(n)
             strides.append(s)
     if len(sizes) > 3 or any(n >= 1 << 31 for n in sizes) or math.prod(sizes[-2:]) >= 1 << 31:
-        return None, None
+        return None
     while len(sizes) < 3:
-        n, s = (sizes[0], strides[0]) if sizes else (1, x.shape[-1])
+        n, s = (sizes[0], strides[0]) if sizes else (1, shape[-1])
         sizes.insert(0, 1)
         strides.insert(0, n * s)
     return sizes, strides
 
 
-def _param(p, c, x, what):
-    if p is None:
+@_signature
+def _ln_fields(shape, stride, dtype):
+    """L.Tensor fields behind the pointer for the rows of such a tensor (last dimension = channels, the others numbered in order), or None:
+    its channels are not adjacent or its leading dimensions do not reduce to three strides"""
+    c = shape[-1]
+    if c > 1 and stride[-1] != 1:
         return None
-    _tensor(p, what, torch.float32, 1)
-    if p.shape[0] != c:
+    lead = _lead(shape, stride)
+    return None if lead is None else (*lead[0][:3], c, *lead[1], L.DT[dtype], 0)
+
+
+@_signature
+def _ln_dense(shape, dtype):
+    """(fields of a contiguous tensor of this shape, rows, channels, bytes of backward scratch)"""
+    if not shape or not 1 <= shape[-1] < 1 << 31:
+        raise L.MyoloError(f'layer_norm: no channels in a tensor of shape {tuple(shape)}')
+    stride, n = [], 1
+    for d in reversed(shape):
+        stride.insert(0, n)
+        n *= max(d, 1)
+    f = _ln_fields(tuple(shape), tuple(stride), dtype)
+    if f is None:
+        raise L.MyoloError('layer_norm: more than 2^31 - 1 rows in one dimension')
+    rows = f[0] * f[1] * f[2]
+    return f, rows, f[3], L.lib().myolo_layernorm_ws_bytes(rows, f[3])
+
+
+def _ln_rows(x):
+    """(tensor to read, its L.Tensor); copied where no descriptor reaches its rows"""
+    f = _ln_fields(x.shape, x.stride(), x.dtype)
+    if f is None:
+        x = x.contiguous()
+        f = _ln_dense(x.shape, x.dtype)[0]
+    return x, L.Tensor(x.data_ptr(), *f)
+
+
+def _param(p, c, what):
+    if p.dtype != torch.float32 or p.dim() != 1 or p.shape[0] != c or not p.is_cuda:
+        _tensor(p, what, torch.float32, 1)
         raise L.MyoloError(f'{what} has {p.shape[0]} values for {c} channels')
-    return p.contiguous()
+    return p if p.is_contiguous() else p.contiguous()
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        lib = L.lib()
-        x, xd = _rows(x)
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        _, od = _rows(out)
-        n, c = xd.n * xd.h * xd.w, xd.c
-        od.n, od.h, od.w, od.sn, od.sh, od.sw = xd.n, xd.h, xd.w, xd.h * xd.w * c, xd.w * c, c
-        train = any(ctx.needs_input_grad[:3])
+    def forward(ctx, x, weight, bias, eps, train):
+        dense, n, c, _ = _ln_dense(x.shape, x.dtype)
+        x, xd = _ln_rows(x)
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        od = L.Tensor(out.data_ptr(), *dense)
+        if xd.n != od.n or xd.h != od.h or xd.w != od.w:         # (the view's dimensions merge less far than the dense result's)
+            od = _like_rows(out, xd)
         saved = torch.empty(2 * n, dtype=torch.float32, device=x.device) if train else None
-        with _on(x):
-            L.check(lib.myolo_layernorm_fwd(C.byref(xd), L.ptr(weight), L.ptr(bias), eps, C.byref(od), L.ptr(saved), L.stream_ptr()),
-                    'myolo_layernorm_fwd')
+        _launch(x.get_device(), 'myolo_layernorm_fwd', C.byref(xd), weight.data_ptr() if weight is not None else None,
+                bias.data_ptr() if bias is not None else None, eps, C.byref(od), saved.data_ptr() if train else None)
         if train:
             ctx.save_for_backward(x, weight, saved)
         return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, go):
-        lib = L.lib()
         x, weight, saved = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        x, xd = _rows(x)
-        go = go.to(x.dtype)
-        if go.shape[-1] > 1 and go.stride(-1) != 1 or _lead(go)[0] != [xd.n, xd.h, xd.w]:
-            go = go.contiguous()
-        n, c = xd.n * xd.h * xd.w, xd.c
-        dense = [xd.h * xd.w * c, xd.w * c, c]
-        gs = dense if go.is_contiguous() else _lead(go)[1]
-        gd = L.Tensor(go.data_ptr(), xd.n, xd.h, xd.w, c, *gs, L.DT[x.dtype], 0)
-        gx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_x else None
-        gxd = L.Tensor(gx.data_ptr(), xd.n, xd.h, xd.w, c, *dense, L.DT[x.dtype], 0) if want_x else None
-        gw = torch.empty(c, dtype=torch.float32, device=x.device) if want_w else None
-        gb = torch.empty(c, dtype=torch.float32, device=x.device) if want_b else None
-        nb = lib.myolo_layernorm_ws_bytes(n, c) if want_w or want_b else 0
-        ws = torch.empty(nb // 4, dtype=torch.float32, device=x.device) if nb else None
-        with _on(x):
-            L.check(lib.myolo_layernorm_bwd(C.byref(gd), C.byref(xd), L.ptr(saved), L.ptr(weight), C.byref(gxd) if want_x else None, 0,
-                                            L.ptr(gw), L.ptr(gb), 0, L.ptr(ws), nb, L.stream_ptr()), 'myolo_layernorm_bwd')
-        return gx, gw, gb, None
+        dense, n, c, nb = _ln_dense(x.shape, x.dtype)
+        dev = x.device
+        x, xd = _ln_rows(x)
+        if go.dtype != x.dtype:
+            go = go.to(x.dtype)
+        go, gd = _ln_rows(go)
+        gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_x else None
+        gxd = L.Tensor(gx.data_ptr() if want_x else None, *dense)
+        if not (xd.n == gd.n == gxd.n and xd.h == gd.h == gxd.h and xd.w == gd.w == gxd.w):
+            gxd = _like_rows(gx, xd) if want_x else gxd
+            if (gd.n, gd.h, gd.w) != (xd.n, xd.h, xd.w):
+                go = go.contiguous()
+                gd = _like_rows(go, xd)
+        gw = torch.empty(c, dtype=torch.float32, device=dev) if want_w else None
+        gb = torch.empty(c, dtype=torch.float32, device=dev) if want_b else None
+        if not (want_w or want_b):
+            nb = 0
+        ws = torch.empty(nb // 4, dtype=torch.float32, device=dev) if nb else None
+        _launch(x.get_device(), 'myolo_layernorm_bwd', C.byref(gd), C.byref(xd), saved.data_ptr(), weight.data_ptr() if weight is not None else None,
+                C.byref(gxd) if want_x else None, 0, gw.data_ptr() if want_w else None, gb.data_ptr() if want_b else None, 0,
+                ws.data_ptr() if nb else None, nb)
+        return gx, gw, gb, None, None
+
+
+def _like_rows(t, d):
+    """the rows of the contiguous tensor t numbered as descriptor d numbers its own"""
+    return L.Tensor(t.data_ptr(), d.n, d.h, d.w, d.c, d.h * d.w * d.c, d.w * d.c, d.c, d.dtype, 0)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) * (var + eps)^-1/2 * weight + bias over the last dimension of x [..., C] (any C >= 1, any strides; a channels-last feature
     map is x.permute(0, 2, 3, 1)).  weight, bias: fp32 [C] or None.  The result is contiguous, in x's dtype; gradients for x, weight, bias."""
     _tensor(x, 'layer_norm: x')
-    if not (isinstance(eps, (int, float)) and eps >= 0.0 and math.isfinite(eps)):
+    if not (isinstance(eps, (int, float)) and 0.0 <= eps < math.inf):
         raise L.MyoloError(f'layer_norm: eps must be a number >= 0, got {eps!r}')
-    c = x.shape[-1] if x.dim() else 0
-    weight, bias = _param(weight, c, x, 'layer_norm: weight'), _param(bias, c, x, 'layer_norm: bias')
-    _same_device(x, weight, bias)
-    return _LayerNorm.apply(x, weight, bias, float(eps))
+    c = _ln_dense(x.shape, x.dtype)[2]
+    if weight is not None:
+        weight = _param(weight, c, 'layer_norm: weight')
+    if bias is not None:
+        bias = _param(bias, c, 'layer_norm: bias')
+    _device(x, weight, bias)
+    return _LayerNorm.apply(x, weight, bias, float(eps), _needs_grad(x, weight, bias))
 
 
 # ---- rotary positions ------------------------------------------------------------------------------------------------------------------
-@functools.lru_cache(maxsize=64)
+@_signature
 def rope_table(sections, theta=10000.0, spectrum='shared'):
     """host table of the rotary pairs: (turns per unit of position, fp64 ctypes array; axis of every pair, int32 ctypes array).  A pure function
     of its arguments.  spectrum 'shared': pair j of all n turns with theta^(-j / n); 'axis': pair j of an axis' n_a with theta^(-j / n_a)."""
-    sections = tuple(sections)
     n = sum(sections)
     turns, axis = [], []
     for a, na in enumerate(sections):
@@ -163,36 +208,65 @@ def rope_table(sections, theta=10000.0, spectrum='shared'):
     return (C.c_double * max(n, 1))(*turns), (C.c_int32 * max(n, 1))(*axis)
 
 
-def _strides(t):
+def _strides(shape, stride):
     """{batch, token, head} strides of [b, l, h, d]; a dimension of one element has none that matters"""
-    return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
+    return [s if n > 1 else 0 for n, s in zip(shape[:3], stride[:3])]
 
 
-def rope_desc(q, k, qo, ko, pos, table, sections, interleaved, inverse):
+def _dense_strides(shape):
+    return _strides(shape, (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3]))
+
+
+@_signature
+def _rope_desc(qshape, qstride, qostride, kshape, kstride, kostride, pshape, pstride, dtype, sections, theta, interleaved, spectrum, inverse):
+    """descriptor without addresses, after all checks"""
+    b, l, hq, dim = qshape
+    if kshape is not None and ((kshape[0], kshape[1], kshape[3]) != (b, l, dim) or kshape[2] < 1):
+        raise L.MyoloError(f'rope_axes: q {tuple(qshape)} and k {tuple(kshape)} differ in more than their heads')
+    if not 1 <= len(sections) <= L.ROPE_MAX_AXES or min(sections) < 0:
+        raise L.MyoloError(f'rope_axes: sections {sections}: 1 to {L.ROPE_MAX_AXES} axes with counts >= 0')
+    if 2 * sum(sections) > dim or sum(sections) > L.ROPE_MAX_PAIRS:
+        raise L.MyoloError(f'rope_axes: {sum(sections)} pairs in {dim} channels (at most {L.ROPE_MAX_PAIRS})')
+    if len(pshape) not in (2, 3) or tuple(pshape[-2:]) != (l, len(sections)) or (len(pshape) == 3 and pshape[0] not in (1, b)):
+        raise L.MyoloError(f'rope_axes: pos {tuple(pshape)} for {l} tokens, {len(sections)} axes and a batch of {b}')
+    if spectrum not in ('shared', 'axis') or not 0.0 < theta < math.inf:
+        raise L.MyoloError(f'rope_axes: spectrum {spectrum!r}, theta {theta!r}')
+    if hq < 1 or dim < 1 or max(b, l, hq, dim) >= 1 << 31:
+        raise L.MyoloError(f'rope_axes: q {tuple(qshape)}')
     d = L.RopeDesc()
-    b, l, hq, dim = q.shape
-    d.q, d.qo, d.pos = q.data_ptr(), qo.data_ptr(), pos.data_ptr()
-    d.qs, d.qos = _P3(*_strides(q)), _P3(*_strides(qo))
-    if k is not None:
-        d.k, d.ko, d.hk = k.data_ptr(), ko.data_ptr(), k.shape[2]
-        d.ks, d.kos = _P3(*_strides(k)), _P3(*_strides(ko))
-    d.ps = _P3(pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0, pos.stride(-2), pos.stride(-1))
-    d.turns, d.axis = C.cast(table[0], C.c_void_p), C.cast(table[1], C.c_void_p)
+    d.qs, d.qos = _P3(*_strides(qshape, qstride)), _P3(*_strides(qshape, qostride))
+    if kshape is not None:
+        d.hk, d.ks, d.kos = kshape[2], _P3(*_strides(kshape, kstride)), _P3(*_strides(kshape, kostride))
+    d.ps = _P3(pstride[0] if len(pshape) == 3 and pshape[0] > 1 else 0, pstride[-2], pstride[-1])
+    turns, axis = rope_table(sections, theta, spectrum)          # (held by rope_call while the call reads them)
     d.b, d.l, d.hq, d.d = b, l, hq, dim
-    d.npair, d.naxis, d.interleaved, d.inverse, d.dtype = sum(sections), len(sections), int(interleaved), int(inverse), L.DT[q.dtype]
-    return d
+    d.npair, d.naxis, d.interleaved, d.inverse, d.dtype = sum(sections), len(sections), int(interleaved), int(inverse), L.DT[dtype]
+    return bytes(d), turns, axis
+
+
+def rope_desc(q, k, qo, ko, pos, spec, inverse):
+    """myolo_rope's descriptor of q, k -> qo, ko (spec: sections, theta, interleaved, spectrum) and what has to outlive the call"""
+    none = (None, None, None)
+    raw, turns, axis = _rope_desc(q.shape, q.stride(), qo.stride(), *((k.shape, k.stride(), ko.stride()) if k is not None else none),
+                                  pos.shape, pos.stride(), q.dtype, *spec, inverse)
+    d = L.RopeDesc.from_buffer_copy(raw)
+    d.q, d.qo, d.pos = q.data_ptr(), qo.data_ptr(), pos.data_ptr()
+    if k is not None:
+        d.k, d.ko = k.data_ptr(), ko.data_ptr()
+    d.turns, d.axis = C.addressof(turns), C.addressof(axis)
+    return d, (turns, axis)
 
 
 def _rope(q, k, pos, spec, inverse):
-    sections, theta, interleaved, spectrum = spec
-    q = q if q.stride(-1) == 1 or q.shape[-1] == 1 else q.contiguous()
+    if q.stride(-1) != 1 and q.shape[-1] > 1:
+        q = q.contiguous()
     qo, ko = torch.empty(q.shape, dtype=q.dtype, device=q.device), None
     if k is not None:
-        k = k if k.stride(-1) == 1 or k.shape[-1] == 1 else k.contiguous()
+        if k.stride(-1) != 1 and k.shape[-1] > 1:
+            k = k.contiguous()
         ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    table = rope_table(sections, theta, spectrum)
-    with _on(q):
-        L.check(L.lib().myolo_rope(C.byref(rope_desc(q, k, qo, ko, pos, table, sections, interleaved, inverse)), L.stream_ptr()), 'myolo_rope')
+    d, keep = rope_desc(q, k, qo, ko, pos, spec, inverse)
+    _launch(q.get_device(), 'myolo_rope', C.byref(d))
     return qo, ko
 
 
@@ -203,8 +277,7 @@ class _Rope(torch.autograd.Function):
         ctx.spec, ctx.like = spec, (q.shape, None if k is None else k.shape, q.dtype, q.device)
         return _rope(q, k, pos, spec, False)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, gq, gk):
         pos, = ctx.saved_tensors
         qs, ks, dt, dev = ctx.like
@@ -225,89 +298,130 @@ def rope_axes(q, k, pos, sections, theta=10000.0, interleaved=False, spectrum='s
     _tensor(q, 'rope_axes: q', dim=4)
     if k is not None:
         _tensor(k, 'rope_axes: k', q.dtype, 4)
-        if (k.shape[0], k.shape[1], k.shape[3]) != (q.shape[0], q.shape[1], q.shape[3]) or k.shape[2] < 1:
-            raise L.MyoloError(f'rope_axes: q {tuple(q.shape)} and k {tuple(k.shape)} differ in more than their heads')
     _tensor(pos, 'rope_axes: pos', torch.int64)
-    _same_device(q, k, pos)
-    sections = tuple(int(s) for s in sections)
-    if not 1 <= len(sections) <= L.ROPE_MAX_AXES or min(sections) < 0:
-        raise L.MyoloError(f'rope_axes: sections {sections}: 1 to {L.ROPE_MAX_AXES} axes with counts >= 0')
-    if 2 * sum(sections) > q.shape[3] or sum(sections) > L.ROPE_MAX_PAIRS:
-        raise L.MyoloError(f'rope_axes: {sum(sections)} pairs in {q.shape[3]} channels (at most {L.ROPE_MAX_PAIRS})')
-    if tuple(pos.shape[-2:]) != (q.shape[1], len(sections)) or pos.dim() not in (2, 3) or (pos.dim() == 3 and pos.shape[0] not in (1, q.shape[0])):
-        raise L.MyoloError(f'rope_axes: pos {tuple(pos.shape)} for {q.shape[1]} tokens, {len(sections)} axes and a batch of {q.shape[0]}')
-    if spectrum not in ('shared', 'axis') or not theta > 0.0:
-        raise L.MyoloError(f'rope_axes: spectrum {spectrum!r}, theta {theta!r}')
-    if q.shape[2] < 1 or q.shape[3] < 1:
-        raise L.MyoloError(f'rope_axes: q {tuple(q.shape)}')
-    return _Rope.apply(q, k, pos, (sections, float(theta), bool(interleaved), spectrum))
+    _device(q, k, pos)
+    spec = (tuple(map(int, sections)), float(theta), bool(interleaved), spectrum)
+    if not _needs_grad(q, k):
+        return _rope(q, k, pos, spec, False)
+    return _Rope.apply(q, k, pos, spec)
 
 
 # ---- attention -------------------------------------------------------------------------------------------------------------------------
-def _side(t):
-    """[b, l, h, d] as the kernels take it: adjacent channels, 16-byte aligned base and strides"""
-    seg = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % seg for s in _strides(t)):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _attn_desc(q, k, v, o, lse, opt):
-    window, sinks, causal, lens, starts, scale = opt
+@_signature
+def _attn_plan(qshape, kshape, vshape, dtype, window, sinks, causal, scale):
+    """(descriptor without addresses and input strides, bytes of forward and of backward scratch), after all checks"""
+    b, lq, hq, dim = qshape
+    lk, hk = kshape[1], kshape[2]
+    if kshape != vshape or kshape[0] != b or kshape[3] != dim:
+        raise L.MyoloError(f'window_attention: q {tuple(qshape)}, k {tuple(kshape)}, v {tuple(vshape)}')
+    if hk < 1 or hq < 1 or hq % hk:
+        raise L.MyoloError(f'window_attention: {hq} query heads over {hk} key heads')
+    if dim % 8 or not 8 <= dim <= ATTN_MAX_DIM:
+        raise L.MyoloError(f'window_attention: head dimension {dim} (a multiple of 8 up to {ATTN_MAX_DIM})')
+    if window < 0 or sinks < 0 or int(window) != window or int(sinks) != sinks:
+        raise L.MyoloError(f'window_attention: window {window}, sinks {sinks}')
+    if max(lq * (hq // hk), lk, window) > L.ATTN_MAX_LEN or b * hq >= 1 << 24:
+        raise L.MyoloError('window_attention: sequence, window or batch too long')
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise L.MyoloError(f'window_attention: scale {scale}')
     d = L.AttnDesc()
-    d.q, d.k, d.v, d.o, d.lse, d.lens, d.starts = (0 if t is None else t.data_ptr() for t in (q, k, v, o, lse, lens, starts))
-    d.qs, d.ks, d.vs, d.os = (_P3(*_strides(t)) for t in (q, k, v, o))
-    d.b, d.lq, d.hq, d.d = q.shape
-    d.lk, d.hk = k.shape[1], k.shape[2]
-    d.dtype, d.causal, d.window, d.sinks, d.scale = L.DT[q.dtype], int(causal), window, sinks, scale
+    d.b, d.lq, d.hq, d.d, d.lk, d.hk = b, lq, hq, dim, lk, hk
+    d.dtype, d.causal, d.window, d.sinks, d.scale = L.DT[dtype], int(bool(causal)), int(window), min(int(sinks), lk), scale
+    for n in ('qs', 'os', 'gos', 'gqs'):
+        setattr(d, n, _P3(*_dense_strides(qshape)))
+    for n in ('ks', 'vs', 'gks', 'gvs'):
+        setattr(d, n, _P3(*_dense_strides(kshape)))
+    return bytes(d), L.lib().myolo_attn_ws_bytes(C.byref(d), 0), L.lib().myolo_attn_ws_bytes(C.byref(d), 1)
+
+
+@_signature
+def _attn_strides(shape, stride, esize):
+    """element strides as the kernels take them, or None: channels not adjacent or rows off a 16-byte boundary"""
+    s = _strides(shape, stride)
+    if (stride[3] != 1 and shape[3] > 1) or any(v * esize % 16 for v in s):
+        return None
+    return _P3(*s)
+
+
+def _side(t):
+    """(tensor, its strides for the descriptor or None where dense); a copy where the kernels cannot read it in place"""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, None
+    s = _attn_strides(t.shape, t.stride(), t.element_size()) if t.data_ptr() % 16 == 0 else None
+    return (t.clone(memory_format=torch.contiguous_format), None) if s is None else (t, s)
+
+
+def _attn_desc(plan, q, k, v, o, lse, lens, starts):
+    d = L.AttnDesc.from_buffer_copy(plan)
+    for t, p, s in ((q, 'q', 'qs'), (k, 'k', 'ks'), (v, 'v', 'vs')):
+        setattr(d, p, t[0].data_ptr())
+        if t[1] is not None:
+            setattr(d, s, t[1])
+    d.o = o.data_ptr()
+    if lse is not None:
+        d.lse = lse.data_ptr()
+    if lens is not None:
+        d.lens = lens.data_ptr()
+    if starts is not None:
+        d.starts = starts.data_ptr()
     return d
 
 
-def _scratch(nbytes, t):
-    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
+def _scratch(d, nbytes, device):
+    if not nbytes:
+        return None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    d.ws, d.ws_bytes = ws.data_ptr(), nbytes
+    return ws
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, opt):
-        lib = L.lib()
+    def forward(ctx, q, k, v, lens, starts, plan, train):
+        raw, nf, _ = plan
         q, k, v = _side(q), _side(k), _side(v)
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        train = any(ctx.needs_input_grad[:3])
-        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if train else None
-        d = _attn_desc(q, k, v, o, lse, opt)
-        d.ws_bytes = lib.myolo_attn_ws_bytes(C.byref(d), 0)
-        ws = _scratch(d.ws_bytes, q)
-        d.ws = ws.data_ptr() if ws is not None else 0
-        with _on(q):
-            L.check(lib.myolo_attn_fwd(C.byref(d), L.stream_ptr()), 'myolo_attn_fwd')
+        dev = q[0].device
+        o = torch.empty(q[0].shape, dtype=q[0].dtype, device=dev)
+        lse = torch.empty(o.shape[0], o.shape[2], o.shape[1], dtype=torch.float32, device=dev) if train else None
+        d = _attn_desc(raw, q, k, v, o, lse, lens, starts)
+        ws = _scratch(d, nf, dev)
+        _launch(o.get_device(), 'myolo_attn_fwd', C.byref(d))
         if train:
-            ctx.save_for_backward(q, k, v, o, lse, opt[3], opt[4])
-            ctx.opt = opt[:3] + (None, None) + opt[5:]
+            ctx.save_for_backward(q[0], k[0], v[0], o, lse, lens, starts)
+            ctx.plan = plan
         return o
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, go):
-        lib = L.lib()
         q, k, v, o, lse, lens, starts = ctx.saved_tensors
-        opt = ctx.opt[:3] + (lens, starts) + ctx.opt[5:]
-        go = _side(go.to(q.dtype))
-        want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        gq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_q else None
-        gk, gv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) if want_kv else None for _ in range(2))
-        d = _attn_desc(q, k, v, o, lse, opt)
-        d.go, d.gos = go.data_ptr(), _P3(*_strides(go))
+        raw, _, nb = ctx.plan
+        if go.dtype != q.dtype:
+            go = go.to(q.dtype)
+        go, gos = _side(go)
+        want_q, want_k, want_v = ctx.needs_input_grad[:3]
+        dev = q.device
+        d = _attn_desc(raw, _side(q), _side(k), _side(v), o, lse, lens, starts)
+        d.go = go.data_ptr()
+        if gos is not None:
+            d.gos = gos
+        gq = gk = gv = None
         if want_q:
-            d.gq, d.gqs = gq.data_ptr(), _P3(*_strides(gq))
-        if want_kv:
-            d.gk, d.gv, d.gks, d.gvs = gk.data_ptr(), gv.data_ptr(), _P3(*_strides(gk)), _P3(*_strides(gv))
-        d.ws_bytes = lib.myolo_attn_ws_bytes(C.byref(d), 1)
-        ws = _scratch(d.ws_bytes, q)
-        d.ws = ws.data_ptr() if ws is not None else 0
-        with _on(q):
-            L.check(lib.myolo_attn_bwd(C.byref(d), L.stream_ptr()), 'myolo_attn_bwd')
-        return gq, gk if ctx.needs_input_grad[1] else None, gv if ctx.needs_input_grad[2] else None, None
+            gq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            d.gq = gq.data_ptr()
+        if want_k or want_v:
+            gk, gv = torch.empty(k.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=q.dtype, device=dev)
+            d.gk, d.gv = gk.data_ptr(), gv.data_ptr()
+        ws = _scratch(d, nb, dev)
+        _launch(q.get_device(), 'myolo_attn_bwd', C.byref(d))
+        return gq, gk if want_k else None, gv if want_v else None, None, None, None, None
+
+
+def _rows32(t, b, what):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != b or not t.is_cuda:
+        _tensor(t, what, torch.int32, 1)
+        raise L.MyoloError(f'{what} has {t.shape[0]} values for a batch of {b}')
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def window_attention(q, k, v, window=0, sinks=0, causal=False, lens=None, starts=None, scale=None):
@@ -323,25 +437,10 @@ def window_attention(q, k, v, window=0, sinks=0, causal=False, lens=None, starts
     _tensor(q, 'window_attention: q', dim=4)
     _tensor(k, 'window_attention: k', q.dtype, 4)
     _tensor(v, 'window_attention: v', q.dtype, 4)
-    b, lq, hq, dim = q.shape
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != dim:
-        raise L.MyoloError(f'window_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}')
-    if k.shape[2] < 1 or hq < 1 or hq % k.shape[2]:
-        raise L.MyoloError(f'window_attention: {hq} query heads over {k.shape[2]} key heads')
-    if dim % 8 or not 8 <= dim <= ATTN_MAX_DIM:
-        raise L.MyoloError(f'window_attention: head dimension {dim} (a multiple of 8 up to {ATTN_MAX_DIM})')
-    if max(lq * (hq // k.shape[2]), k.shape[1], window) > L.ATTN_MAX_LEN or b * hq >= 1 << 24:
-        raise L.MyoloError('window_attention: sequence, window or batch too long')
-    if window < 0 or sinks < 0 or int(window) != window or int(sinks) != sinks:
-        raise L.MyoloError(f'window_attention: window {window}, sinks {sinks}')
-    for t, n in ((lens, 'lens'), (starts, 'starts')):
-        if t is not None:
-            _tensor(t, 'window_attention: ' + n, torch.int32, 1)
-            if t.shape[0] != b:
-                raise L.MyoloError(f'window_attention: {n} has {t.shape[0]} values for a batch of {b}')
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise L.MyoloError(f'window_attention: scale {scale}')
-    _same_device(q, k, v, lens, starts)
-    lens, starts = (None if t is None else t.contiguous() for t in (lens, starts))
-    return _WindowAttention.apply(q, k, v, (int(window), min(int(sinks), k.shape[1]), bool(causal), lens, starts, scale))
+    plan = _attn_plan(q.shape, k.shape, v.shape, q.dtype, window, sinks, causal, scale)
+    if lens is not None:
+        lens = _rows32(lens, q.shape[0], 'window_attention: lens')
+    if starts is not None:
+        starts = _rows32(starts, q.shape[0], 'window_attention: starts')
+    _device(q, k, v, lens, starts)
+    return _WindowAttention.apply(q, k, v, lens, starts, plan, _needs_grad(q, k, v))

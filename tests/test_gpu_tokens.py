@@ -195,7 +195,7 @@ def test_rope_c_entry_in_place():
     pos = torch.randint(0, 90, (2, 11, 2), generator=torch.Generator().manual_seed(3))
     for sections in ((8, 16), (3, 4)):
         qd, kd, pd = cuda(q, k, pos)
-        d = T().rope_desc(qd, kd, qd, kd, pd, T().rope_table(sections), sections, False, False)
+        d, keep = T().rope_desc(qd, kd, qd, kd, pd, (sections, 10000.0, False, 'shared'), False)
         assert L.lib().myolo_rope(C.byref(d), L.stream_ptr()) == 0
         R.within('q', qd, *R.rope(q, pos, sections, 10000.0, False, 'shared'))
         R.within('k', kd, *R.rope(k, pos, sections, 10000.0, False, 'shared'))
