@@ -736,14 +736,17 @@ KvShape kv_shape(const myolo_attn_desc* d) {
   const int64_t full = (d->lq + bq - 1) / bq * g, total = bh * k.nblk;
   if (!total || !full) return k;
   int64_t n = 1;
-  if (d->window && d->sinks) {          // a block of sinks walks every query, its neighbours the band: cut it to their length
+  if (d->window && d->sinks) {          // a block of sinks walks every query, its neighbours the band: cut it to quarters of their length
     const int64_t band = (((int64_t)d->window * (d->causal ? 1 : 2) + 127) / bq + 2) * g;
-    n = (full + band - 1) / band;
-    if (n > 1) k.nsb = (int)(((d->sinks < d->lk ? d->sinks : d->lk) + 127) / 128);
+    if (full > band) {
+      n = (4 * full + band - 1) / band;
+      k.nsb = (int)(((d->sinks < d->lk ? d->sinks : d->lk) + 127) / 128);
+    }
   }
-  if (total < 512) {                    // fewer than two workgroups a CU: every block is shared
+  const int64_t fill = d->d <= 64 ? 512 : 256;           // workgroups that are resident at once
+  if (total < fill) {                   // CUs would idle: every block is shared
     k.nsb = k.nblk;
-    const int64_t w = (512 + total - 1) / total;
+    const int64_t w = (fill + total - 1) / total;
     if (w > n) n = w;
   }
   if (n > full) n = full;

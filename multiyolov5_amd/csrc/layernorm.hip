@@ -147,14 +147,26 @@ template <typename T, int VEC, int NV> struct RowRegs {
 };
 template <int VEC, int NV> struct ParamRegs {
   float v[NV * VEC];
+  // (16-byte loads where the parameter vector allows them: 4 lanes' worth of scalar loads would outnumber the row's own)
   __device__ __forceinline__ void load(const float* p, int t, int g, int c, float none) {
+    const bool al = VEC > 1 && ((uintptr_t)p & 15) == 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * g + t) * VEC;
+      const bool ok = p && col < c;
+      if (al) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int col = (i * g + t) * VEC + e;
-        v[i * VEC + e] = p ? (col < c ? p[col] : 0.f) : none;
+        for (int e = 0; e < VEC; e += 4) {
+          const uint4 q = ldg16(ok ? (const char*)(p + col + e) : zero_page());
+          const float* f = reinterpret_cast<const float*>(&q);
+#pragma unroll
+          for (int k = 0; k < (VEC > 1 ? 4 : 1); ++k) v[i * VEC + e + k] = p ? f[k] : none;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i * VEC + e] = p ? (ok ? p[col + e] : 0.f) : none;
       }
+    }
   }
 };
 // sum over the G lanes of a row (WIDE: over the workgroup)
@@ -358,6 +370,12 @@ __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* ws, 
   }
 }
 
+#ifndef LN_GRID
+#define LN_GRID 1024
+#endif
+#ifndef LN_MAXNV
+#define LN_MAXNV 4
+#endif
 // how a row is laid out over lanes: vectors a lane, lanes a row (log2), or the whole workgroup; nv == 0: read row by row (any_kernel)
 struct Lay { int nv, glog; bool wide; };
 Lay lay_of(int c, int vec) {
@@ -367,7 +385,7 @@ Lay lay_of(int c, int vec) {
   Lay best{0, 0, false};
   int waste = 1 << 30;
   for (int gl = 6; gl >= 2; --gl)
-    for (int nv = 1; nv <= 4; ++nv)
+    for (int nv = 1; nv <= LN_MAXNV; ++nv)
       if ((nv << gl) >= n && (nv << gl) - n < waste) { waste = (nv << gl) - n; best = Lay{nv, gl, false}; }
   if (best.nv) return best;
   if (vec < 8 && n <= 64 * 8) return Lay{8, 6, false};
@@ -419,7 +437,7 @@ int ln_fwd(const myolo_tensor* x, const float* gamma, const float* beta, float e
     hipLaunchKernelGGL((ln_fwd_any_kernel<T, VEC>), dim3(grid), dim3(256), 0, st, rx, ro, rows, x->c, gamma, beta, eps, saved);
   } else {
     const int64_t per = l.wide ? 1 : 1 << (8 - l.glog), all = (rows + per - 1) / per;
-    const int grid = (int)(all < 2048 ? all : 2048);
+    const int grid = (int)(all < LN_GRID ? all : LN_GRID);
 #define LN_FWD(NV, WIDE) \
   hipLaunchKernelGGL((ln_fwd_kernel<T, VEC, NV, WIDE>), dim3(grid), dim3(256), 0, st, rx, ro, rows, x->c, l.glog, gamma, beta, eps, saved)
     LN_BY_NV(LN_FWD)

@@ -54,66 +54,103 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a) {
   }
 }
 
-// Vector path: a thread owns one 16-byte unit of pairs of one token (SEG pairs (j, j + npair) in two vectors, or SEG / 2 neighbouring pairs in
-// one) and HC of its heads: the angles are formed once for all of them, behind loads that are already in flight.  Adjacent lanes take
-// adjacent units, then adjacent heads: a wave's accesses are contiguous.  Units behind the pairs copy the pass-through channels.
-template <typename T, bool IL, int HC>
-__global__ __launch_bounds__(256) void rope_vec_kernel(RopeArgs a, int units, int pass, int hl) {
-  constexpr int SEG = ET<T>::SEG, NP = IL ? SEG / 2 : SEG, NV = IL ? 1 : 2;
-  const int per = (units + pass) * hl, heads = a.s[0].h + a.s[1].h;
-  const int64_t total = a.tokens * per;
-  for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < total; w += (int64_t)gridDim.x * 256) {
-    const int64_t tok = w / per, b = tok / a.l, i = tok - b * a.l;
-    const int q = (int)(w - tok * per), h0 = q / (units + pass), un = q - h0 * (units + pass);
-    const int c0 = un < units ? un * SEG : 2 * a.npair + (un - units) * SEG;       // (first channel; the pair's second vector: + npair)
-    uint4 in[HC][NV];
-    char* op[HC];
+// Vector path: a workgroup owns tb tokens.  It forms their sines and cosines once, in LDS, for all heads, behind the loads of what they will
+// turn: a thread owns one 16-byte unit of pairs (SEG pairs (j, j + npair) in two vectors, or SEG / 2 neighbouring pairs in one) of HC heads of
+// q or of k.  Adjacent lanes take adjacent units, then other heads of the token: HBM sees whole lines.  Units behind the pairs copy the
+// pass-through channels.
+template <typename T, bool IL, int HC> struct RopeItem {
+  static constexpr int SEG = ET<T>::SEG, NP = IL ? SEG / 2 : SEG, NV = IL ? 1 : 2;
+  uint4 in[HC][NV];
+  char* o;
+  int64_t ostep;
+  int tl, un, n;           // token in the workgroup, unit, heads
+
+  // item it of the workgroup: chunk ch < nq takes heads ch, ch + nq, ... of q, the others likewise of k
+  __device__ __forceinline__ void load(const RopeArgs& a, int it, int units, int upt, int nq, int nch, int b, int i0) {
+    const int per = upt * nch;
+    tl = it / per;
+    const int rem = it - tl * per, c = rem / upt;
+    un = rem - c * upt;
+    const bool isq = c < nq;
+    const int h0 = isq ? c : c - nq, step = isq ? nq : nch - nq, heads = isq ? a.s[0].h : a.s[1].h;
+    const int64_t i = i0 + tl;
+    const int c0 = (un < units ? un * SEG : 2 * a.npair + (un - units) * SEG) * (int)sizeof(T);
+    const char* x = isq ? a.s[0].x + (b * a.s[0].sb + i * a.s[0].sl + h0 * a.s[0].sh) : a.s[1].x + (b * a.s[1].sb + i * a.s[1].sl + h0 * a.s[1].sh);
+    o = isq ? a.s[0].o + (b * a.s[0].ob + i * a.s[0].ol + h0 * a.s[0].oh) : a.s[1].o + (b * a.s[1].ob + i * a.s[1].ol + h0 * a.s[1].oh);
+    const int64_t xstep = step * (isq ? a.s[0].sh : a.s[1].sh);
+    ostep = step * (isq ? a.s[0].oh : a.s[1].oh);
+    x += c0;
+    o += c0;
+    n = (heads - h0 + step - 1) / step;
 #pragma unroll
     for (int k = 0; k < HC; ++k) {
-      const int h = h0 + k * hl, kh = h - a.s[0].h;
-      const RopeSide& s = kh < 0 ? a.s[0] : a.s[1];
-      const int hh = kh < 0 ? h : kh;
-      const bool ok = h < heads;
-      const char* x = s.x + b * s.sb + i * s.sl + hh * s.sh + c0 * (int)sizeof(T);
-      op[k] = ok ? s.o + b * s.ob + i * s.ol + hh * s.oh + c0 * (int)sizeof(T) : nullptr;
-      in[k][0] = ldg16(ok ? x : zero_page());
-      if constexpr (!IL) in[k][1] = ldg16(ok && un < units ? x + a.npair * (int)sizeof(T) : zero_page());
+      const char* xk = k < n ? x + k * xstep : zero_page();
+      in[k][0] = ldg16(xk);
+      if constexpr (!IL) in[k][1] = ldg16((k < n) & (un < units) ? xk + a.npair * (int)sizeof(T) : zero_page());
     }
+  }
+  __device__ __forceinline__ void turn(const RopeArgs& a, const float2* tab, int units) const {
     if (un >= units) {
 #pragma unroll
       for (int k = 0; k < HC; ++k)
-        if (op[k]) stg16(op[k], in[k][0]);
-      continue;
+        if (k < n) stg16(o + k * ostep, in[k][0]);
+      return;
     }
-    float sn[NP], cs[NP];
-    const int64_t* pos = a.pos + b * a.pb + i * a.pl;
+    float2 sc[NP];
 #pragma unroll
-    for (int e = 0; e < NP; ++e) turn_of(a, pos, un * NP + e, sn + e, cs + e);
+    for (int e = 0; e < NP; ++e) sc[e] = tab[tl * a.npair + un * NP + e];
 #pragma unroll
     for (int k = 0; k < HC; ++k) {
-      if (!op[k]) continue;
+      if (k >= n) break;
       float u[SEG];
       Vec<T>::unpack(in[k][0], u);
       if constexpr (IL) {
 #pragma unroll
         for (int e = 0; e < NP; ++e) {
           const float x = u[2 * e], y = u[2 * e + 1];
-          u[2 * e] = x * cs[e] - y * sn[e];
-          u[2 * e + 1] = y * cs[e] + x * sn[e];
+          u[2 * e] = x * sc[e].y - y * sc[e].x;
+          u[2 * e + 1] = y * sc[e].y + x * sc[e].x;
         }
-        stg16(op[k], Vec<T>::pack(u));
+        stg16(o + k * ostep, Vec<T>::pack(u));
       } else {
         float v[SEG];
         Vec<T>::unpack(in[k][1], v);
 #pragma unroll
         for (int e = 0; e < NP; ++e) {
           const float x = u[e], y = v[e];
-          u[e] = x * cs[e] - y * sn[e];
-          v[e] = y * cs[e] + x * sn[e];
+          u[e] = x * sc[e].y - y * sc[e].x;
+          v[e] = y * sc[e].y + x * sc[e].x;
         }
-        stg16(op[k], Vec<T>::pack(u));
-        stg16(op[k] + a.npair * (int)sizeof(T), Vec<T>::pack(v));
+        stg16(o + k * ostep, Vec<T>::pack(u));
+        stg16(o + k * ostep + a.npair * (int)sizeof(T), Vec<T>::pack(v));
       }
+    }
+  }
+};
+
+constexpr int kTable = 2048;         // (sine, cosine) entries of a workgroup: 16 KB
+
+template <typename T, bool IL, int HC>
+__global__ __launch_bounds__(256) void rope_vec_kernel(RopeArgs a, int units, int pass, int nq, int nch, int tb, int nb) {
+  __shared__ float2 tab[kTable];
+  const int upt = units + pass, per = upt * nch;
+  const int64_t i0 = (int64_t)blockIdx.x * tb;
+  const int nt = (int)min((int64_t)tb, a.l - i0), items = nt * per;
+  for (int b = blockIdx.y; b < nb; b += gridDim.y) {
+    RopeItem<T, IL, HC> cur;
+    if (threadIdx.x < items) cur.load(a, threadIdx.x, units, upt, nq, nch, b, (int)i0);
+    if (b != (int)blockIdx.y) __syncthreads();
+    const int64_t* pos = a.pos + b * a.pb + i0 * a.pl;
+    for (int e = threadIdx.x; e < nt * a.npair; e += 256) {
+      const int t = e / a.npair, j = e - t * a.npair;
+      float sn, cs;
+      turn_of(a, pos + t * a.pl, j, &sn, &cs);
+      tab[e] = float2{sn, cs};
+    }
+    __syncthreads();
+    for (int it = threadIdx.x; it < items; it += 256) {
+      if (it != (int)threadIdx.x) cur.load(a, it, units, upt, nq, nch, b, (int)i0);
+      cur.turn(a, tab, units);
     }
   }
 }
@@ -132,18 +169,20 @@ template <typename T> int run_rope(const RopeArgs& a, hipStream_t st) {
     MYOLO_CHECK_LAUNCH();
     return 0;
   }
-  const int units = a.npair / np, pass = (a.d - 2 * a.npair) / SEG;
-  // four heads a thread where that still leaves four waves for every CU's SIMD, one where the call is that small
-  const int hc = a.tokens * heads * (units + pass) >= 4 * 4 * 256 * 256 ? 4 : 1;
-  const int hl = (heads + hc - 1) / hc;
-  const int grid = grid_for(a.tokens * hl * (units + pass), 256, 1 << 20);
-  if (a.interleaved) {
-    if (hc == 4) hipLaunchKernelGGL((rope_vec_kernel<T, true, 4>), dim3(grid), dim3(256), 0, st, a, units, pass, hl);
-    else hipLaunchKernelGGL((rope_vec_kernel<T, true, 1>), dim3(grid), dim3(256), 0, st, a, units, pass, hl);
-  } else {
-    if (hc == 4) hipLaunchKernelGGL((rope_vec_kernel<T, false, 4>), dim3(grid), dim3(256), 0, st, a, units, pass, hl);
-    else hipLaunchKernelGGL((rope_vec_kernel<T, false, 1>), dim3(grid), dim3(256), 0, st, a, units, pass, hl);
-  }
+  const int units = a.npair / np, pass = (a.d - 2 * a.npair) / SEG, upt = units + pass;
+  // four heads a thread where that still leaves sixteen waves for every CU, one where the call is that small
+  const int hc = a.tokens * heads * upt >= 4 * 16 * 256 * 64 ? 4 : 1;
+  const int nq = (a.s[0].h + hc - 1) / hc, nch = nq + (a.s[1].h + hc - 1) / hc, per = upt * nch;
+  int tb = 256 / per;                                    // one item a thread; a token at least
+  if (tb < 1) tb = 1;
+  if (tb > a.l) tb = a.l;
+  while (tb > 1 && tb * a.npair > kTable) --tb;          // (npair <= 128: one token always fits)
+  const int nb = (int)(a.tokens / a.l);
+  const dim3 grid((unsigned)((a.l + tb - 1) / tb), (unsigned)(nb < 65535 ? nb : 65535));
+#define ROPE(IL, HC) hipLaunchKernelGGL((rope_vec_kernel<T, IL, HC>), grid, dim3(256), 0, st, a, units, pass, nq, nch, tb, nb)
+  if (a.interleaved) { if (hc == 4) ROPE(true, 4); else ROPE(true, 1); }
+  else { if (hc == 4) ROPE(false, 4); else ROPE(false, 1); }
+#undef ROPE
   MYOLO_CHECK_LAUNCH();
   return 0;
 }
