@@ -944,6 +944,127 @@ class DropoutOp(SimpleOp):
                                                          self.acc)))
 
 
+class LayerNormOp(SimpleOp):
+    """layer norm over the channels of every pixel; `norm`: an nn.LayerNorm used as a parameter container"""
+
+    def __init__(self, plan, src, dst, norm):
+        super().__init__(plan, src, dst)
+        if tuple(norm.normalized_shape) != (src.c,):
+            raise L.MyoloError(f'LayerNorm over {tuple(norm.normalized_shape)} of a map of {src.c} channels')
+        self.norm = norm
+
+    def build(self, plan):
+        n, c = self.src.n * self.src.h * self.src.w, self.src.c
+        w, b = self.norm.weight, self.norm.bias
+        if w is not None and w.dtype != torch.float32:        # .half() model (eval): the kernel reads fp32 copies, refreshed by prepare()
+            self.w32 = torch.empty(c, dtype=torch.float32, device=plan.device)
+            self.b32 = torch.empty(c, dtype=torch.float32, device=plan.device) if b is not None else None
+        self.gamma, self.beta = (self.w32, self.b32) if hasattr(self, 'w32') else (w, b)
+        self.saved = torch.zeros(2 * n, dtype=torch.float32, device=plan.device) if plan.training else None
+        super().build(plan)
+        if plan.training and not self.src.requires_grad and w is not None:
+            self.gdd = self.dst.desc(grad=True)
+            self.emit_bwd(plan)
+
+    def prepare(self):
+        if hasattr(self, 'w32'):
+            with torch.no_grad():
+                self.w32.copy_(self.norm.weight)
+                if self.b32 is not None:
+                    self.b32.copy_(self.norm.bias)
+
+    def emit_fwd(self, plan):
+        self.fwd_calls.append(Call('myolo_layernorm_fwd', (C.byref(self.sd), L.ptr(self.gamma), L.ptr(self.beta), C.c_float(self.norm.eps),
+                                                           C.byref(self.dd), L.ptr(self.saved)), keep=self.norm))
+
+    def emit_bwd(self, plan):
+        nb = L.lib().myolo_layernorm_ws_bytes(self.src.n * self.src.h * self.src.w, self.src.c)
+        self.ws = torch.empty(max(nb // 4, 1), dtype=torch.float32, device=plan.device)
+        self.bwd_calls.append(Call('myolo_layernorm_bwd', (
+            C.byref(self.gdd), C.byref(self.sd), L.ptr(self.saved), L.ptr(self.gamma), C.byref(self.gsd) if self.src.requires_grad else None, self.acc,
+            L.ptr(plan.pgrad(self.norm.weight)), L.ptr(plan.pgrad(self.norm.bias)), 1, L.ptr(self.ws), nb)))
+
+
+def _token_strides(d, head):
+    """{batch, token, head} strides of a view's pixels as tokens in raster order (every Buf is dense in y)"""
+    assert d.sh == d.w * d.sw
+    return (C.c_int64 * 3)(d.sn, d.sw, head)
+
+
+class RopeOp(Op):
+    """rotary positions of a map's pixels (height, width) on the heads of q and k: out views, so that v stays where the projection wrote it"""
+
+    def __init__(self, plan, q, k, oq, ok, dim, sections, theta):
+        from .utils import tokens
+        self.q, self.k, self.oq, self.ok, self.dim, self.sections = q, k, oq, ok, dim, sections
+        self.table = tokens.rope_table(tuple(sections), float(theta), 'axis')
+
+    def grad_io(self):
+        return [self.oq, self.ok], [self.q, self.k]
+
+    def plan_bwd(self, plan):
+        for tv in (self.q, self.k):
+            acc, z = claim(tv)
+            assert not acc and not z, 'a projection has a single consumer'
+
+    def _desc(self, plan, src, dst, inverse):
+        (qd, kd), (oq, ok) = src, dst
+        d = L.RopeDesc()
+        d.q, d.k, d.qo, d.ko, d.pos = qd.ptr, kd.ptr, oq.ptr, ok.ptr, self.pos.data_ptr()
+        d.qs, d.ks, d.qos, d.kos = (_token_strides(t, self.dim) for t in (qd, kd, oq, ok))
+        d.ps = (C.c_int64 * 3)(0, 2, 1)
+        d.turns, d.axis = C.addressof(self.table[0]), C.addressof(self.table[1])
+        d.b, d.l, d.hq, d.hk, d.d = qd.n, qd.h * qd.w, qd.c // self.dim, kd.c // self.dim, self.dim
+        d.npair, d.naxis, d.inverse, d.dtype = sum(self.sections), 2, inverse, qd.dtype
+        return d
+
+    def build(self, plan):
+        super().build(plan)
+        y, x = torch.meshgrid(torch.arange(self.q.h), torch.arange(self.q.w), indexing='ij')
+        self.pos = torch.stack([y, x], -1).reshape(-1, 2).contiguous().to(plan.device)
+        self.fd = self._desc(plan, (self.q.desc(), self.k.desc()), (self.oq.desc(), self.ok.desc()), 0)
+        self.fwd_calls.append(Call('myolo_rope', (C.byref(self.fd),)))
+        if plan.training:
+            self.bd = self._desc(plan, (self.oq.desc(grad=True), self.ok.desc(grad=True)), (self.q.desc(grad=True), self.k.desc(grad=True)), 1)
+            self.bwd_calls.append(Call('myolo_rope', (C.byref(self.bd),)))
+
+
+class WindowAttnOp(Op):
+    """attention between a map's pixels in raster order: a pixel sees the pixels less than `window` away (0: all) and the first `sinks`"""
+
+    def __init__(self, plan, q, k, v, out, dim, window, sinks):
+        self.q, self.k, self.v, self.out, self.dim, self.window, self.sinks = q, k, v, out, dim, window, sinks
+
+    def grad_io(self):
+        return [self.out], [self.q, self.k, self.v]
+
+    def plan_bwd(self, plan):
+        for tv in (self.q, self.k, self.v):
+            acc, z = claim(tv)
+            assert not acc and not z, 'a projection has a single consumer'
+
+    def build(self, plan):
+        super().build(plan)
+        q, k, v, o = (t.desc() for t in (self.q, self.k, self.v, self.out))
+        d = self.d = L.AttnDesc()
+        n = q.h * q.w
+        d.q, d.k, d.v, d.o = q.ptr, k.ptr, v.ptr, o.ptr
+        d.qs, d.ks, d.vs, d.os = (_token_strides(t, self.dim) for t in (q, k, v, o))
+        d.b, d.lq, d.lk, d.hq, d.hk, d.d, d.dtype = q.n, n, n, q.c // self.dim, k.c // self.dim, self.dim, q.dtype
+        d.window, d.sinks, d.scale = self.window, self.sinks, self.dim ** -0.5
+        nb = [L.lib().myolo_attn_ws_bytes(C.byref(d), i) for i in range(2 if plan.training else 1)]
+        self.ws = torch.empty(max(nb + [16]), dtype=torch.uint8, device=plan.device)     # (forward and backward of an op never overlap)
+        d.ws, d.ws_bytes = self.ws.data_ptr(), self.ws.numel()
+        if plan.training:
+            self.lse = torch.zeros(q.n * d.hq * n, dtype=torch.float32, device=plan.device)
+            d.lse = self.lse.data_ptr()
+            g = [t.desc(grad=True) for t in (self.out, self.q, self.k, self.v)]
+            d.go, d.gq, d.gk, d.gv = (t.ptr for t in g)
+            d.gos, d.gqs, d.gks, d.gvs = (_token_strides(t, self.dim) for t in g)
+            self.bwd_calls.append(Call('myolo_attn_bwd', (C.byref(d),)))
+        self.fwd_calls.append(Call('myolo_attn_fwd', (C.byref(d),)))
+
+
 class AddOp(Op):
     """out = a + b (BiSe `m16 + feat3`, yolo.py:84)."""
 

@@ -515,3 +515,60 @@ class ARM(PlannedModule):
         out = plan.new(feat.n, feat.h, feat.w, feat.c)
         plan.add(E.GateOp(plan, feat, a, out, residual=False))
         return out
+
+
+class AttnLayer(PlannedModule):
+    """Transformer layer over the pixels of a map, tokens in raster order (the reference's TransformerLayer, common.py:49-63, mixes pixels by
+    nn.MultiheadAttention without norm or positions): x + proj(attention(q, k, v of LN(x))), then that + fc2(SiLU(fc1(LN))).
+
+    q and k carry rotary positions of (height, width).  `rows`: a pixel sees the pixels less than `rows` map rows away in raster order
+    (0: the whole map), so the cost grows with the map's width instead of its area; `sinks`: the first pixels, which every pixel sees as
+    well.  `num_kv_heads` < `num_heads`: key / value heads shared by groups of query heads."""
+
+    def __init__(self, c, num_heads=4, num_kv_heads=None, rows=0, sinks=0, mlp=2, theta=100.0):
+        super().__init__()
+        kv = num_kv_heads or num_heads
+        if c % num_heads or (c // num_heads) % 8 or c // num_heads > 128 or num_heads % kv:
+            raise ValueError(f'AttnLayer: {num_heads} / {kv} heads in {c} channels (a head is a multiple of 8 channels, at most 128)')
+        self.dim, self.heads, self.kv, self.rows, self.sinks, self.theta = c // num_heads, num_heads, kv, int(rows), int(sinks), theta
+        self.norm1 = nn.LayerNorm(c)
+        self.qkv = nn.Conv2d(c, (num_heads + 2 * kv) * self.dim, 1)
+        self.proj = nn.Conv2d(c, c, 1)
+        self.norm2 = nn.LayerNorm(c)
+        self.fc1 = nn.Conv2d(c, mlp * c, 1, bias=False)
+        self.fc2 = nn.Conv2d(mlp * c, c, 1)
+
+    def emit(self, plan, x):
+        def norm(t, m):
+            y = plan.new(t.n, t.h, t.w, t.c)
+            plan.add(E.LayerNormOp(plan, t, y, m))
+            return y
+
+        def add(a, b):
+            y = plan.new(a.n, a.h, a.w, a.c)
+            plan.add(E.AddOp(plan, a, b, y))
+            return y
+
+        def view(buf, c0, c):
+            t = plan.new(x.n, x.h, x.w, c)
+            t.place(buf, c0)
+            return t
+        d, hq, hk = self.dim, self.heads * self.dim, self.kv * self.dim
+        buf, turned = plan.new_buf(x.n, x.h, x.w, hq + 2 * hk), plan.new_buf(x.n, x.h, x.w, hq + hk)
+        emit_conv(plan, norm(x, self.norm1), self.qkv, out=view(buf, 0, hq + 2 * hk))
+        q, k = view(turned, 0, hq), view(turned, hq, hk)
+        plan.add(E.RopeOp(plan, view(buf, 0, hq), view(buf, hq, hk), q, k, d, (d // 4, d // 4), self.theta))
+        o = plan.new(x.n, x.h, x.w, hq)
+        plan.add(E.WindowAttnOp(plan, q, k, view(buf, hq + hk, hk), o, d, self.rows * x.w, self.sinks))
+        y = add(x, emit_conv(plan, o, self.proj)[0])
+        t = emit_conv(plan, norm(y, self.norm2), self.fc1, act=SILU)[0]
+        return add(y, emit_conv(plan, t, self.fc2)[0])
+
+
+class C3Attn(C3):
+    """C3 (common.py:127-139) whose inner blocks are transformer layers"""
+
+    def __init__(self, c1, c2, n=1, num_heads=4, rows=0, sinks=0, e=0.5):
+        super().__init__(c1, c2, 0, e=e)
+        c_ = int(c2 * e)
+        self.m = nn.Sequential(*[AttnLayer(c_, num_heads, rows=rows, sinks=sinks) for _ in range(n)])

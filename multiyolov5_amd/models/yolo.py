@@ -322,12 +322,12 @@ def parse_model(d, ch):                                        # yolo.py:373-429
             except Exception:
                 pass
         n = max(round(n * gd), 1) if n > 1 else n
-        if m in [Conv, SPP, Focus, C3, ASPP]:
+        if m in [Conv, SPP, Focus, C3, C3Attn, ASPP]:
             c1, c2 = ch[f], args[0]
             if c2 != no:
                 c2 = make_divisible(c2 * gw, 8)
             args = [c1, c2, *args[1:]]
-            if m is C3:
+            if m in (C3, C3Attn):
                 args.insert(2, n)
                 n = 1
         elif m is Concat:
