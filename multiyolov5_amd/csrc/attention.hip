@@ -121,6 +121,28 @@ template <typename T, int DL> struct Tile {
   }
 };
 
+// the column operands of 32 rows from r0 on, 32 columns a step (two 16-row operands): AHEAD reads step m + 1 before step m's matrix
+// instructions are issued and keeps the scheduler from moving the reads back to their use
+template <typename T, int DL, bool AHEAD> struct Columns {
+  const uint4* s;
+  int r0, lane;
+  Frag<T> f[AHEAD ? 2 : 1][2];
+  __device__ __forceinline__ Columns(const uint4* s_, int r0_, int lane_) : s(s_), r0(r0_), lane(lane_) {}
+  __device__ __forceinline__ void read(int m) {
+    Tile<T, DL>::col_frag(f[AHEAD ? m & 1 : 0][0], s, r0, m * 32, lane);
+    Tile<T, DL>::col_frag(f[AHEAD ? m & 1 : 0][1], s, r0 + 16, m * 32, lane);
+  }
+  __device__ __forceinline__ void first() { if constexpr (AHEAD) read(0); }
+  __device__ __forceinline__ void next(int m) { if constexpr (AHEAD) read(m + 1); }
+  __device__ __forceinline__ void now(int m) {
+    if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+    else read(m);
+  }
+  __device__ __forceinline__ const Frag<T>& a(int m) const { return f[AHEAD ? m & 1 : 0][0]; }
+  __device__ __forceinline__ const Frag<T>& b(int m) const { return f[AHEAD ? m & 1 : 0][1]; }
+};
+template <typename T> constexpr bool kAheadOf = sizeof(T) == 2;
+
 // the value of the lane's column in the other half of the wave, combined
 __device__ __forceinline__ float half_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -274,15 +296,17 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
     gk.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.d, tid, ok);
     gv.load(vp + (int64_t)j0 * a.vs[1], a.vs[1], a.d, tid, ok);
   };
-  if (t0 < t1) fetch(t0);
-  for (int t = t0; t < t1; ++t) {
-    const int j0 = tl.at(t) * BK;
-    if (t > t0) __syncthreads();
+  auto put = [&]() {
     gk.template store<DL>(sK, tid);
     gv.template store<DL>(sV, tid);
+  };
+  if (t0 < t1) { fetch(t0); put(); }
+  for (int t = t0; t < t1; ++t) {
+    const int j0 = tl.at(t) * BK;
+    const bool more = t + 1 < t1;
     __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
-    if (!vis.any(pw0, pw1, j0, j0 + BK - 1)) continue;
+    if (more) fetch(t + 1);
+    if (vis.any(pw0, pw1, j0, j0 + BK - 1)) {
     f16_t s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -336,6 +360,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
         o[m] = mma(vf, p1, o[m]);
       }
     }
+    }
+    __syncthreads();
+    if (more) put();
   }
   l = half_sum(l);
   if (!live) return;
@@ -415,6 +442,7 @@ constexpr float kPShift = 12.f, kPUnshift = 1.f / 4096.f;
 
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
+  constexpr bool kAhead = kAheadOf<T> && DP <= 64;         // (more: spills at two waves a SIMD)
   constexpr int NW = 4, BK = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
   using TL = Tile<T, DL>;
   __shared__ uint4 sK[BK * TL::CH], sV[BK * TL::CH];
@@ -467,44 +495,64 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
     gk.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.d, tid, ok);
     gv.load(vp + (int64_t)j0 * a.vs[1], a.vs[1], a.d, tid, ok);
   };
-  if (nt) fetch(0);
-  for (int t = 0; t < nt; ++t) {
-    const int j0 = tl.at(t) * BK;
-    if (t) __syncthreads();
+  auto put = [&]() {
     gk.template store<DL>(sK, tid);
     gv.template store<DL>(sV, tid);
+  };
+  if (nt) { fetch(0); put(); }
+  for (int t = 0; t < nt; ++t) {
+    const int j0 = tl.at(t) * BK;
+    const bool more = t + 1 < nt;
     __syncthreads();
-    if (t + 1 < nt) fetch(t + 1);
-    if (!vis.any(pw0, pw1, j0, j0 + BK - 1)) continue;
+    if (more) fetch(t + 1);
+    if (vis.any(pw0, pw1, j0, j0 + BK - 1)) {
     const bool all = vis.all(pw0, pw1, j0, j0 + BK - 1);
 #pragma unroll
     for (int u = 0; u < BK / 32; ++u) {
       f16_t s = f16_t{}, dp = f16_t{};
+      if constexpr (kAhead) {
+        Frag<T> fk[KS], fv[KS];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        Frag<T> f;
-        TL::row_frag(f, sK, u * 32 + (lane & 31), k * 2 + h);
-        s = mma(f, qf[k], s);
-        TL::row_frag(f, sV, u * 32 + (lane & 31), k * 2 + h);
-        dp = mma(f, gf[k], dp);
+        for (int k = 0; k < KS; ++k) TL::row_frag(fk[k], sK, u * 32 + (lane & 31), k * 2 + h);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) TL::row_frag(fv[k], sV, u * 32 + (lane & 31), k * 2 + h);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) s = mma(fk[k], qf[k], s);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) dp = mma(fv[k], gf[k], dp);
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          Frag<T> f;
+          TL::row_frag(f, sK, u * 32 + (lane & 31), k * 2 + h);
+          s = mma(f, qf[k], s);
+          TL::row_frag(f, sV, u * 32 + (lane & 31), k * 2 + h);
+          dp = mma(f, gf[k], dp);
+        }
       }
+      Columns<T, DL, kAhead> ck(sK, u * 32, lane);
+      ck.first();
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, -lse)) * (dp[r] - delta);
       if (!all) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = lkeys.has(j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[r] : 0.f;
       }
-      Frag<T> d0, d1, kf;
+      Frag<T> d0, d1;
       frag_from<0>(d0, s);
       frag_from<1>(d1, s);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        TL::col_frag(kf, sK, u * 32, m * 32, lane);
-        dq[m] = mma(kf, d0, dq[m]);
-        TL::col_frag(kf, sK, u * 32 + 16, m * 32, lane);
-        dq[m] = mma(kf, d1, dq[m]);
+        if (m + 1 < MT) ck.next(m);
+        ck.now(m);
+        dq[m] = mma(ck.a(m), d0, dq[m]);
+        dq[m] = mma(ck.b(m), d1, dq[m]);
       }
     }
+    }
+    __syncthreads();
+    if (more) put();
   }
   if (!live || !a.gq) return;
   char* dp = a.gq + b * a.gqs[0] + qi * a.gqs[1] + head * a.gqs[2];
@@ -524,6 +572,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
 // a fixed order.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
+  constexpr bool kAhead = kAheadOf<T>;
   constexpr int NW = 4, BQ = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
   using TL = Tile<T, DL>;
   __shared__ uint4 sQ[BQ * TL::CH], sG[BQ * TL::CH];
@@ -586,69 +635,89 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_
       nd = on ? a.delta[lr] * kPUnshift : 0.f;
     }
   };
-  if (t0 < t1) fetch(t0);
-  for (int t = t0; t < t1; ++t) {
-    const int hd = t / nq, i0 = (q0 + t - hd * nq) * BQ;
-    if (t > t0) __syncthreads();
+  auto put = [&]() {
     gq.template store<DL>(sQ, tid);
     gg.template store<DL>(sG, tid);
     if (tid < BQ) { sL[tid] = nl; sD[tid] = nd; }
+  };
+  if (t0 < t1) { fetch(t0); put(); }
+  for (int t = t0; t < t1; ++t) {
+    const int hd = t / nq, i0 = (q0 + t - hd * nq) * BQ;
+    const bool more = t + 1 < t1;
     __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
+    if (more) fetch(t + 1);
     const int p0 = vis.start + i0, p1 = p0 + BQ - 1;
-    if (kw0 > kw1 || !vis.any(p0, p1, kw0, kw1)) continue;
+    if ((kw0 <= kw1) & vis.any(p0, p1, kw0, kw1)) {
     const bool all = kw0 + 31 < a.lk && i0 + BQ <= a.lq && vis.all(p0, p1, kw0, kw1);
 #pragma unroll 1
     for (int u = 0; u < BQ / 32; ++u) {
+      // fp16: the row operands of both products are read ahead of their matrix instructions, the column operands a step ahead, so that exp
+      // runs beside the second product and dS beside dv (fp32 operands are twice the registers and a sixteenth of the rate: read in place)
       f16_t s = f16_t{}, dp = f16_t{};
+      if constexpr (kAhead) {
+        Frag<T> fq[KS], fg[KS];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        Frag<T> f;
-        TL::row_frag(f, sQ, u * 32 + (lane & 31), k * 2 + h);
-        s = mma(f, kf[k], s);
-        TL::row_frag(f, sG, u * 32 + (lane & 31), k * 2 + h);
-        dp = mma(f, vf[k], dp);
+        for (int k = 0; k < KS; ++k) TL::row_frag(fq[k], sQ, u * 32 + (lane & 31), k * 2 + h);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) TL::row_frag(fg[k], sG, u * 32 + (lane & 31), k * 2 + h);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) s = mma(fq[k], kf[k], s);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) dp = mma(fg[k], vf[k], dp);
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          Frag<T> f;
+          TL::row_frag(f, sQ, u * 32 + (lane & 31), k * 2 + h);
+          s = mma(f, kf[k], s);
+          TL::row_frag(f, sG, u * 32 + (lane & 31), k * 2 + h);
+          dp = mma(f, vf[k], dp);
+        }
       }
+      Columns<T, DL, kAhead> cg(sG, u * 32, lane), cq(sQ, u * 32, lane);
+      cg.first();
+      f4_t l4[4], d4[4];
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const int qb = u * 32 + 8 * r4 + 4 * h;
-        const f4_t l4 = *reinterpret_cast<const f4_t*>(sL + qb), d4 = *reinterpret_cast<const f4_t*>(sD + qb);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * r4 + e;
-          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, l4[e]));
-          dp[r] = s[r] * fmaf(dp[r], kPUnshift, -d4[e]);
-        }
+        l4[r4] = *reinterpret_cast<const f4_t*>(sL + u * 32 + 8 * r4 + 4 * h);
+        d4[r4] = *reinterpret_cast<const f4_t*>(sD + u * 32 + 8 * r4 + 4 * h);
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, l4[r >> 2][r & 3]));
       if (!all) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int q = u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
-          const bool on = lrows.has(p0 + q);
-          s[r] = on ? s[r] : 0.f;
-          dp[r] = on ? dp[r] : 0.f;
-        }
+        for (int r = 0; r < 16; ++r) s[r] = lrows.has(p0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[r] : 0.f;
       }
-      Frag<T> f0, f1, c;
+      Frag<T> f0, f1;
       frag_from<0>(f0, s);
       frag_from<1>(f1, s);
 #pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = s[r] * fmaf(dp[r], kPUnshift, -d4[r >> 2][r & 3]);
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = lrows.has(p0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? dp[r] : 0.f;
+      }
+#pragma unroll
       for (int m = 0; m < MT; ++m) {
-        TL::col_frag(c, sG, u * 32, m * 32, lane);
-        dv[m] = mma(f0, c, dv[m]);
-        TL::col_frag(c, sG, u * 32 + 16, m * 32, lane);
-        dv[m] = mma(f1, c, dv[m]);
+        if (m + 1 < MT) cg.next(m); else cq.first();
+        cg.now(m);
+        dv[m] = mma(f0, cg.a(m), dv[m]);
+        dv[m] = mma(f1, cg.b(m), dv[m]);
       }
       frag_from<0>(f0, dp);
       frag_from<1>(f1, dp);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        TL::col_frag(c, sQ, u * 32, m * 32, lane);
-        dk[m] = mma(f0, c, dk[m]);
-        TL::col_frag(c, sQ, u * 32 + 16, m * 32, lane);
-        dk[m] = mma(f1, c, dk[m]);
+        if (m + 1 < MT) cq.next(m);
+        cq.now(m);
+        dk[m] = mma(f0, cq.a(m), dk[m]);
+        dk[m] = mma(f1, cq.b(m), dk[m]);
       }
     }
+    }
+    __syncthreads();
+    if (more) put();
   }
   // accumulators: column (lane % 32) = channel, rows = keys
   const int col = lane & 31;
@@ -688,6 +757,7 @@ __global__ __launch_bounds__(256) void attn_bwd_kv_join_kernel(AttnArgs a) {
     if (kk >= a.lk) continue;
     const float* p = a.part + bb * a.nsplit * 2 * 128 * a.d + (int64_t)which * 128 * a.d + kr * a.d + c;
     f4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int i = 0; i < a.nsplit; ++i) s += *reinterpret_cast<const f4_t*>(p + (int64_t)i * 2 * 128 * a.d);
     const float f = which ? kPUnshift : a.scale;
     T* g = which ? (T*)(a.gv + b * a.gvs[0] + kh * a.gvs[2] + (int64_t)kk * a.gvs[1]) : (T*)(a.gk + b * a.gks[0] + kh * a.gks[2] + (int64_t)kk * a.gks[1]);
@@ -736,14 +806,16 @@ KvShape kv_shape(const myolo_attn_desc* d) {
   const int64_t full = (d->lq + bq - 1) / bq * g, total = bh * k.nblk;
   if (!total || !full) return k;
   int64_t n = 1;
-  if (d->window && d->sinks) {          // a block of sinks walks every query, its neighbours the band: cut it to quarters of their length
+  const int64_t fill = d->d <= 64 ? 512 : 256;           // workgroups that are resident at once
+  if (d->window && d->sinks) {
+    // a block of sinks walks every query, its neighbours the band.  Cut it to the band's length where several rounds of workgroups follow it,
+    // to eighths of that where the last round would wait for it (8 x 32 blocks of 128 channels: 300 -> 271 us; 64 x 16 blocks of 64: 92 -> 98)
     const int64_t band = (((int64_t)d->window * (d->causal ? 1 : 2) + 127) / bq + 2) * g;
     if (full > band) {
-      n = (4 * full + band - 1) / band;
+      n = ((total < 2 * fill ? 8 : 1) * full + band - 1) / band;
       k.nsb = (int)(((d->sinks < d->lk ? d->sinks : d->lk) + 127) / 128);
     }
   }
-  const int64_t fill = d->d <= 64 ? 512 : 256;           // workgroups that are resident at once
   if (total < fill) {                   // CUs would idle: every block is shared
     k.nsb = k.nblk;
     const int64_t w = (fill + total - 1) / total;
