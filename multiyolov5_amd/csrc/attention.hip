@@ -406,33 +406,59 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
     }
 }
 
-// joins the splits of a row: o = sum o_s 2^(m_s - M) / sum l_s 2^(m_s - M)
+// joins the splits of a row: o = sum o_s 2^(m_s - M) / sum l_s 2^(m_s - M).  A workgroup per row: one wave forms the weights (a lane a split),
+// then 8 x 32 threads take every eighth split of four channels; the sums meet in LDS in a fixed order.  (One thread a channel group over all
+// splits took 12 us for 256 rows x 16 splits: a chain of loads.)
+constexpr int kMaxSplit = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-  const int64_t nrow = (int64_t)a.b * a.hk * a.rows, total = nrow * (a.d / 4);
+  __shared__ float sw[kMaxSplit];
+  __shared__ f4_t so[8][32];
+  __shared__ float sinv;
+  const int64_t nrow = (int64_t)a.b * a.hk * a.rows;
   const float* ml = a.part + (int64_t)a.nsplit * nrow * a.d;
-  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
-    const int64_t pr = v / (a.d / 4);
-    const int c = (int)(v - pr * (a.d / 4)) * 4;
-    float mx = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) mx = fmaxf(mx, ml[(s * nrow + pr) * 2]);
-    const float use = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f;
-    f4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float w = __builtin_amdgcn_exp2f(ml[(s * nrow + pr) * 2] - use);
-      l += w * ml[(s * nrow + pr) * 2 + 1];
-      const f4_t x = *reinterpret_cast<const f4_t*>(a.part + (s * nrow + pr) * a.d + c);
+  const int cg = threadIdx.x & 31, sg = threadIdx.x >> 5, c = cg * 4;
+  for (int64_t pr = blockIdx.x; pr < nrow; pr += gridDim.x) {
+    f4_t x[kMaxSplit / 8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += w * x[e];
+    for (int i = 0; i < kMaxSplit / 8; ++i) {
+      const int s = sg + 8 * i;
+      const bool on = (s < a.nsplit) & (c < a.d);
+      const uint4 v = ldg16(on ? (const char*)(a.part + (s * nrow + pr) * a.d + c) : zero_page());
+      x[i] = *reinterpret_cast<const f4_t*>(&v);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
     const int bh = (int)(pr / a.rows), row = (int)(pr - (int64_t)bh * a.rows), b = bh / a.hk;
     const int qi = row / a.g, head = (bh - b * a.hk) * a.g + row - qi * a.g;
-    if (a.lse && c == 0) a.lse[((int64_t)b * a.hq + head) * a.lq + qi] = l == 0.f ? -INFINITY : mx + __log2f(l);
-    T* op = (T*)(a.o + b * a.os[0] + qi * a.os[1] + head * a.os[2]) + c;
+    if (threadIdx.x < 64) {
+      const int s = threadIdx.x;
+      const bool on = s < a.nsplit;
+      const float m = on ? ml[(s * nrow + pr) * 2] : -INFINITY, l = on ? ml[(s * nrow + pr) * 2 + 1] : 0.f;
+      float mx = m;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) op[e] = (T)(o[e] * inv);
+      for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+      const float w = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.f : mx)), sum = wave_sum(w * l);
+      sw[s] = w;
+      if (s == 0) {
+        sinv = sum == 0.f ? 0.f : 1.f / sum;
+        if (a.lse) a.lse[((int64_t)b * a.hq + head) * a.lq + qi] = sum == 0.f ? -INFINITY : mx + __log2f(sum);
+      }
+    }
+    __syncthreads();
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kMaxSplit / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += sw[sg + 8 * i] * x[i][e];
+    so[sg][cg] = o;
+    __syncthreads();
+    if (sg == 0 && c < a.d) {
+#pragma unroll
+      for (int k = 1; k < 8; ++k) o += so[k][cg];
+      T* op = (T*)(a.o + b * a.os[0] + qi * a.os[1] + head * a.os[2]) + c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) op[e] = (T)(o[e] * sinv);
+    }
+    __syncthreads();
   }
 }
 
@@ -794,7 +820,7 @@ FwdShape fwd_shape(const myolo_attn_desc* d) {
   const int64_t tiles = (span + 63) / 64, want = 1024 / f.nw, have = bh * f.nblk;
   int64_t n = have > 0 ? want / have : 1;
   if (n > tiles) n = tiles;
-  if (n > 64) n = 64;
+  if (n > kMaxSplit) n = kMaxSplit;
   f.nsplit = n < 2 ? 1 : (int)n;
   return f;
 }
@@ -851,8 +877,7 @@ int launch_fwd(const AttnArgs& a, hipStream_t st) {
   if (a.nsplit > 1) {
     hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, true>), grid, dim3(NW * 64), 0, st, a);
     MYOLO_CHECK_LAUNCH();
-    const int64_t total = (int64_t)a.b * a.hk * a.rows * (a.d / 4);
-    hipLaunchKernelGGL((attn_join_kernel<T>), dim3(grid_for(total, 256, 4096)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_join_kernel<T>), dim3(grid_for((int64_t)a.b * a.hk * a.rows, 1, 1 << 16)), dim3(256), 0, st, a);
   } else {
     hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, false>), grid, dim3(NW * 64), 0, st, a);
   }
