@@ -169,10 +169,40 @@ template <int VEC, int NV> struct ParamRegs {
     }
   }
 };
-// sum over the G lanes of a row (WIDE: over the workgroup)
-template <bool WIDE> __device__ __forceinline__ float row_sum(float v, int g, float* sm) {
+// sums over the 2^glog lanes of a row (WIDE: over the workgroup), both at once, in every lane.  Lane exchanges of the vector unit (quad
+// permutes, mirrors of 8 and 16 lanes, row swaps): shuffles through LDS cost ten round trips a row, which is what bounded the backward
+// (131072 rows of 192 channels: 42 -> 36 us)
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float swap16_add(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float swap32_add(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <bool WIDE> __device__ __forceinline__ void row_sums(float& a, float& b, int glog, float* sm) {
+  if constexpr (WIDE) {
+    a = block_sum<256>(a, sm);
+    b = block_sum<256>(b, sm);
+    return;
+  }
+  a = dpp_add<0x4e>(dpp_add<0xb1>(a));                     // (groups have at least 4 lanes)
+  b = dpp_add<0x4e>(dpp_add<0xb1>(b));
+  if (glog >= 3) { a = dpp_add<0x141>(a); b = dpp_add<0x141>(b); }
+  if (glog >= 4) { a = dpp_add<0x140>(a); b = dpp_add<0x140>(b); }
+  if (glog >= 5) { a = swap16_add(a); b = swap16_add(b); }
+  if (glog >= 6) { a = swap32_add(a); b = swap32_add(b); }
+}
+template <bool WIDE> __device__ __forceinline__ float row_sum(float v, int glog, float* sm) {
   if constexpr (WIDE) return block_sum<256>(v, sm);
-  for (int o = g >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  v = dpp_add<0x4e>(dpp_add<0xb1>(v));
+  if (glog >= 3) v = dpp_add<0x141>(v);
+  if (glog >= 4) v = dpp_add<0x140>(v);
+  if (glog >= 5) v = swap16_add(v);
+  if (glog >= 6) v = swap32_add(v);
   return v;
 }
 
@@ -200,7 +230,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(Rows x, Rows o, int64_t row
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s += f[i * VEC + e];
     }
-    const float mu = row_sum<WIDE>(s, g, sm) / fc;
+    const float mu = row_sum<WIDE>(s, glog, sm) / fc;
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -210,7 +240,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(Rows x, Rows o, int64_t row
         v = (i * g + t) * VEC < c ? v - mu : 0.f;
         s += v * v;
       }
-    const float rstd = 1.f / sqrtf(row_sum<WIDE>(s, g, sm) / fc + eps);
+    const float rstd = 1.f / sqrtf(row_sum<WIDE>(s, glog, sm) / fc + eps);
     if (r < rows) {
       if (saved && t == 0) { saved[r] = mu; saved[rows + r] = rstd; }
       T* op = row_ptr<T>(o, r);
@@ -272,8 +302,9 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(Rows go, Rows x, Rows gx, i
       }
     }
     if (want_gx) {
-      s1 = row_sum<WIDE>(s1, g, sm) / fc;
-      s2 = row_sum<WIDE>(s2, g, sm) / fc;
+      row_sums<WIDE>(s1, s2, glog, sm);
+      s1 /= fc;
+      s2 /= fc;
       if (r < rows) {
         T* op = row_ptr<T>(gx, r);
 #pragma unroll
@@ -370,23 +401,19 @@ __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* ws, 
   }
 }
 
-#ifndef LN_GRID
-#define LN_GRID 1024
-#endif
-#ifndef LN_MAXNV
-#define LN_MAXNV 4
-#endif
 // how a row is laid out over lanes: vectors a lane, lanes a row (log2), or the whole workgroup; nv == 0: read row by row (any_kernel)
 struct Lay { int nv, glog; bool wide; };
-Lay lay_of(int c, int vec) {
+// most: vectors a lane may hold while its row has lanes left to spread over.  The forward takes up to four (rows of 192: 8 lanes x 3 vectors, no
+// lane idle: 22 us against 39 with 32 lanes x 1), the backward, seven registers an element, needs the waves more than the lanes (36 against 49)
+Lay lay_of(int c, int vec, int most = 4) {
   const int n = (c + vec - 1) / vec;
   // the fewest idle lanes of 4 .. 64 times 1 .. 4 vectors, the most lanes where that ties; then whole waves with more, then workgroups; at
   // most 32 elements a lane (the backward holds seven registers an element: 64 of them spill)
   Lay best{0, 0, false};
   int waste = 1 << 30;
   for (int gl = 6; gl >= 2; --gl)
-    for (int nv = 1; nv <= LN_MAXNV; ++nv)
-      if ((nv << gl) >= n && (nv << gl) - n < waste) { waste = (nv << gl) - n; best = Lay{nv, gl, false}; }
+    for (int nv = 1; nv <= 4; ++nv)
+      if ((nv <= most || gl == 6) && (nv << gl) >= n && (nv << gl) - n < waste) { waste = (nv << gl) - n; best = Lay{nv, gl, false}; }
   if (best.nv) return best;
   if (vec < 8 && n <= 64 * 8) return Lay{8, 6, false};
   if (vec == 1 && n <= 64 * 16) return Lay{16, 6, false};
@@ -397,7 +424,8 @@ Lay lay_of(int c, int vec) {
   return best;
 }
 constexpr int kSlices = 1024;
-// workgroups of the backward (= partial parameter sums): four a CU, each lane group at least four rows
+// workgroups of the backward (= partial parameter sums): four a CU, each lane group at least four rows (131072 x 192: 512 / 768 / 1024 / 1280
+// workgroups take 47 / 39 / 36 / 35 us, their sums another 4.0 / 4.6 / 5.2 / 5.8)
 int bwd_groups(int64_t rows, const Lay& l) {
   const int64_t per = l.wide ? 1 : 1 << (8 - l.glog);
   int64_t n = (rows + per * 4 - 1) / (per * 4);
@@ -437,7 +465,7 @@ int ln_fwd(const myolo_tensor* x, const float* gamma, const float* beta, float e
     hipLaunchKernelGGL((ln_fwd_any_kernel<T, VEC>), dim3(grid), dim3(256), 0, st, rx, ro, rows, x->c, gamma, beta, eps, saved);
   } else {
     const int64_t per = l.wide ? 1 : 1 << (8 - l.glog), all = (rows + per - 1) / per;
-    const int grid = (int)(all < LN_GRID ? all : LN_GRID);
+    const int grid = (int)(all < 1024 ? all : 1024);
 #define LN_FWD(NV, WIDE) \
   hipLaunchKernelGGL((ln_fwd_kernel<T, VEC, NV, WIDE>), dim3(grid), dim3(256), 0, st, rx, ro, rows, x->c, l.glog, gamma, beta, eps, saved)
     LN_BY_NV(LN_FWD)
@@ -454,7 +482,7 @@ int ln_bwd(const myolo_tensor* gout, const myolo_tensor* x, const float* saved, 
   const Rows rx = rows_of(*x), rg = rows_of(*gout), ro = gx ? rows_of(*gx) : Rows{};
   const bool param = dgamma || dbeta;
   const int c = x->c;
-  const Lay l = lay_of(c, VEC);
+  const Lay l = lay_of(c, VEC, 1);
   int ns = 0;
   if (rows && l.nv) {
     ns = bwd_groups(rows, l);
