@@ -7,11 +7,33 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'lib', 'libmyolo.so')
+EXT = os.path.join(HERE, 'lib', '_token_autograd.so')           # autograd nodes of utils/tokens.py (host C++ over the C ABI)
+EXT_SRC = os.path.join(CSRC, 'token_autograd.cpp')
 ARCH = 'gfx950'
 
 
 def sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.hip'))
+
+
+def stale_ext():
+    hdr = os.path.join(os.path.dirname(HERE), 'include', 'myolo.h')
+    return not os.path.exists(EXT) or os.path.getmtime(EXT) < max(os.path.getmtime(EXT_SRC), os.path.getmtime(hdr))
+
+
+def build_ext(verbose=True):
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    inc = include_paths() + ['/opt/rocm/include', sysconfig.get_paths()['include']]
+    cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-D__HIP_PLATFORM_AMD__=1', '-DTORCH_EXTENSION_NAME=_token_autograd',
+           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}'] + [f'-I{p}' for p in inc] + [EXT_SRC] + \
+        [f'-L{p}' for p in library_paths()] + ['-ltorch_python', '-ltorch', '-ltorch_cpu', '-lc10', '-lc10_hip', '-o', EXT]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    if r.returncode != 0:
+        raise RuntimeError('%s\n%s' % (' '.join(cmd), r.stdout.decode()))
+    if verbose:
+        print('built', EXT)
 
 
 def stale():
@@ -31,6 +53,9 @@ PER_FILE_FLAGS = {'augment.hip': ['-ffp-contract=off']}
 
 
 def build(force=False, verbose=True):
+    if force or stale_ext():
+        os.makedirs(os.path.dirname(EXT), exist_ok=True)
+        build_ext(verbose)
     if not force and not stale():
         return LIB
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')

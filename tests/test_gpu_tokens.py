@@ -195,7 +195,13 @@ def test_rope_c_entry_in_place():
     pos = torch.randint(0, 90, (2, 11, 2), generator=torch.Generator().manual_seed(3))
     for sections in ((8, 16), (3, 4)):
         qd, kd, pd = cuda(q, k, pos)
-        d, keep = T().rope_desc(qd, kd, qd, kd, pd, (sections, 10000.0, False, 'shared'), False)
+        turns, axis = T().rope_table(sections)
+        d = L.RopeDesc()
+        d.q, d.qo, d.k, d.ko, d.pos = qd.data_ptr(), qd.data_ptr(), kd.data_ptr(), kd.data_ptr(), pd.data_ptr()
+        d.qs = d.qos = (C.c_int64 * 3)(*qd.stride()[:3])
+        d.ks = d.kos = (C.c_int64 * 3)(*kd.stride()[:3])
+        d.ps, d.turns, d.axis = (C.c_int64 * 3)(*pd.stride()), C.addressof(turns), C.addressof(axis)
+        d.b, d.l, d.hq, d.hk, d.d, d.npair, d.naxis, d.dtype = 2, 11, 3, 1, 48, sum(sections), 2, L.DT[F16]
         assert L.lib().myolo_rope(C.byref(d), L.stream_ptr()) == 0
         R.within('q', qd, *R.rope(q, pos, sections, 10000.0, False, 'shared'))
         R.within('k', kd, *R.rope(k, pos, sections, 10000.0, False, 'shared'))
@@ -449,7 +455,8 @@ def test_chain_matches_the_definitions():
     got = [got, *torch.autograd.grad(got, dl, go.cuda())]
     for n, a, r in zip(('o', 'gx', 'gw', 'gb', 'gwqkv'), got, ref):
         # 32-bit chain of five operators, each good to some tens of 2^-24 of its inputs' size (test_* above): 2^-24 * 1000 of the norm
-        assert float((a.detach().double().cpu() - r).norm()) <= 1000 * R.E * float(r.detach().norm()), n
+        r = r.detach()
+        assert float((a.detach().double().cpu() - r).norm()) <= 1000 * R.E * float(r.norm()), n
 
 
 def test_on_another_stream_and_captured():
@@ -517,6 +524,28 @@ def test_captured_decode_follows_the_lengths():
         R.within('first graph', o1, *ref)
         g2.replay()
         R.within('second graph', o2, *ref)
+
+
+def test_first_derivatives_only_and_saved_tensors_are_guarded():
+    t = T()
+    x, pos = torch.randn(1, 4, 2, 16, device='cuda', requires_grad=True), torch.zeros(4, 1, dtype=torch.int64, device='cuda')
+    for f in (lambda: t.layer_norm(x), lambda: t.rope_axes(x, None, pos, (8,))[0], lambda: t.window_attention(x, x, x)):
+        with pytest.raises(RuntimeError, match='second derivative'):
+            torch.autograd.grad(f().sum(), x, create_graph=True)
+    y = x.detach().clone().requires_grad_()
+    z = y * 1.0
+    out = t.layer_norm(z)
+    z.add_(1.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        out.sum().backward()
+    with torch.inference_mode():
+        assert not t.window_attention(x, x, x).requires_grad
+    assert not t.layer_norm(x.detach()).requires_grad
+    out = t.window_attention(x, x, x)                       # one leaf in three places
+    g, = torch.autograd.grad(out.sum(), x)
+    parts = [x.detach().clone().requires_grad_() for _ in range(3)]
+    gs = torch.autograd.grad(t.window_attention(*parts).sum(), parts)
+    assert torch.equal(g, gs[0] + gs[1] + gs[2]) or torch.allclose(g, gs[0] + gs[1] + gs[2], rtol=4 * R.E, atol=1e-6)
 
 
 # ---- refusals --------------------------------------------------------------------------------------------------------------------------
