@@ -447,14 +447,15 @@ int myolo_rope(const myolo_rope_desc* d, void* stream);
  *   o = softmax over the visible keys of scale * q.k, times v; a query that sees nothing gives 0.
  * Keys that no query of the call sees are never read into a result, whatever they hold.  lens, starts: device int32[b].
  * lse: fp32 [b, hq, lq] (log2 of the softmax denominator of scale*log2(e)*q.k), written by the forward when not NULL, read by the
- * backward.  scale > 0.
+ * backward.  o_res (fp16, laid out like o; may be NULL, NULL for fp32): what the rounding of o left over, written by the forward, read by the
+ * backward, whose row sums of go * o would otherwise carry o's rounding into gq and gk.  scale > 0.
  * ws: myolo_attn_ws_bytes(d, backward) bytes of scratch, 16-byte aligned (0: none needed), free again when the call's work has run.
  * Backward: go = d loss / d o; gq, gk, gv are overwritten (each may be NULL: not wanted; gk and gv are wanted together).  No atomics:
  * results do not depend on the order in which workgroups run. */
 #define MYOLO_ATTN_MAX_LEN (1 << 28)
 typedef struct myolo_attn_desc {
   const void *q, *k, *v;
-  void* o;
+  void *o, *o_res;
   float* lse;
   const int32_t *lens, *starts;
   const void* go;

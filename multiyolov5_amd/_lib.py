@@ -126,7 +126,7 @@ ROPE_MAX_PAIRS, ROPE_MAX_AXES = 128, 4      # MYOLO_ROPE_MAX_PAIRS, MYOLO_ROPE_M
 
 class AttnDesc(C.Structure):
     """myolo_attn_desc (include/myolo.h)"""
-    _fields_ = [('q', C.c_void_p), ('k', C.c_void_p), ('v', C.c_void_p), ('o', C.c_void_p), ('lse', C.c_void_p), ('lens', C.c_void_p),
+    _fields_ = [('q', C.c_void_p), ('k', C.c_void_p), ('v', C.c_void_p), ('o', C.c_void_p), ('o_res', C.c_void_p), ('lse', C.c_void_p), ('lens', C.c_void_p),
                 ('starts', C.c_void_p), ('go', C.c_void_p), ('gq', C.c_void_p), ('gk', C.c_void_p), ('gv', C.c_void_p), ('ws', C.c_void_p),
                 ('ws_bytes', C.c_int64), ('qs', C.c_int64 * 3), ('ks', C.c_int64 * 3), ('vs', C.c_int64 * 3), ('os', C.c_int64 * 3),
                 ('gos', C.c_int64 * 3), ('gqs', C.c_int64 * 3), ('gks', C.c_int64 * 3), ('gvs', C.c_int64 * 3),

@@ -19,7 +19,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnArgs {
   const char *q, *k, *v, *go;
-  char *o, *gq, *gk, *gv;
+  char *o, *ores, *gq, *gk, *gv;
   float *lse, *delta;
   float* part;             // split forward: [split][b*hk][rows][d] unnormalised sums, then [split][b*hk][rows][2] max and denominator
                            // split dk / dv: [b*hk][nsb][split][dk, dv][128][d] partial sums
@@ -143,6 +143,10 @@ template <typename T, int DL, bool AHEAD> struct Columns {
 };
 template <typename T> constexpr bool kAheadOf = sizeof(T) == 2;
 
+// a product as a 32-bit value: without this the compiler rounds it straight to fp16 on the paths that need nothing else of it, and results with
+// and without the residual differ in the last bit
+__device__ __forceinline__ float pin(float x) { asm("" : "+v"(x)); return x; }
+
 // the value of the lane's column in the other half of the wave, combined
 __device__ __forceinline__ float half_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -249,7 +253,7 @@ __device__ __forceinline__ int xcd_order(int id, int n) {
 // ---- forward -------------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
-  constexpr int BK = sizeof(T) == 2 || NW > 1 ? 64 : 32, U = BK / 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
+  constexpr int BK = sizeof(T) == 2 || NW > 1 ? 64 : 32, U = BK / 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = (DP + 31) / 32;
   using TL = Tile<T, DL>;
   __shared__ uint4 sK[BK * TL::CH], sV[BK * TL::CH];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
@@ -393,10 +397,15 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
       const int c = m * 32 + q4 * 8 + 4 * h;
       if (c >= a.d) continue;
       if constexpr (sizeof(T) == 2) {
-        h4_t v;
+        h4_t v, w;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (half_t)(o[m][4 * q4 + e] * inv);
+        for (int e = 0; e < 4; ++e) {
+          const float x = pin(o[m][4 * q4 + e] * inv);
+          v[e] = (half_t)x;
+          w[e] = (half_t)(x - (float)v[e]);
+        }
         *reinterpret_cast<h4_t*>(op + c * 2) = v;
+        if (a.ores) *reinterpret_cast<h4_t*>(a.ores + (op - a.o) + c * 2) = w;
       } else {
         f4_t v;
 #pragma unroll
@@ -456,7 +465,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
       for (int k = 1; k < 8; ++k) o += so[k][cg];
       T* op = (T*)(a.o + b * a.os[0] + qi * a.os[1] + head * a.os[2]) + c;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) op[e] = (T)(o[e] * sinv);
+      for (int e = 0; e < 4; ++e) {
+        const float x = pin(o[e] * sinv);
+        const T v = (T)x;
+        op[e] = v;
+        if (a.ores) ((T*)(a.ores + ((char*)op - a.o)))[e] = (T)(x - (float)v);
+      }
     }
     __syncthreads();
   }
@@ -469,11 +483,13 @@ constexpr float kPShift = 12.f, kPUnshift = 1.f / 4096.f;
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
   constexpr bool kAhead = kAheadOf<T> && DP <= 64;         // (more: spills at two waves a SIMD)
-  constexpr int NW = 4, BK = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
+  constexpr int NW = 4, BK = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = (DP + 31) / 32;
   using TL = Tile<T, DL>;
   __shared__ uint4 sK[BK * TL::CH], sV[BK * TL::CH];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int id = xcd_order(blockIdx.x, gridDim.x);
+  int id = xcd_order(blockIdx.x, gridDim.x);
+  const int sp = id % a.nsplit;                             // few blocks over a long key axis: its tiles are shared, the sums joined
+  id /= a.nsplit;
   const int blk = a.nblk - 1 - id % a.nblk, bh = id / a.nblk;
   const int b = bh / a.hk, kh = bh - b * a.hk;
   const Vis vis = vis_of(a, b);
@@ -500,11 +516,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
     frag_global(gf[s], gp + c * sizeof(T), ok);
     frag_global(of, op + c * sizeof(T), ok);
     delta += frag_dot(gf[s], of);
+    if (a.ores) {
+      frag_global(of, a.ores + (op - a.o) + c * sizeof(T), ok);
+      delta += frag_dot(gf[s], of);
+    }
   }
   delta = half_sum(delta);
   const int64_t lrow = ((int64_t)b * a.hq + head) * a.lq + qi;
   const float lse = a.lse[lrow];
-  if (live && h == 0) a.delta[lrow] = delta;
+  if (live && h == 0 && sp == 0) a.delta[lrow] = delta;
   const char* kp = a.k + b * a.ks[0] + kh * a.ks[2];
   const char* vp = a.v + b * a.vs[0] + kh * a.vs[2];
   f16_t dq[MT];
@@ -513,7 +533,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
 
   const TileList tl = tiles_of(vis, pb0, pb1, BK);
   const Keys bkeys = vis.keys(pb0, pb1), lkeys = vis.keys(p, p);       // the workgroup's keys, the lane's
-  const int nt = a.gq ? tl.n : 0;
+  const int per = (tl.n + a.nsplit - 1) / a.nsplit, t0 = min(sp * per, tl.n), nt = a.gq ? min(t0 + per, tl.n) : t0;
   Stage<T, DP, BK, NT> gk, gv;
   auto fetch = [&](int t) {
     const int j0 = tl.at(t) * BK;
@@ -525,8 +545,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
     gk.template store<DL>(sK, tid);
     gv.template store<DL>(sV, tid);
   };
-  if (nt) { fetch(0); put(); }
-  for (int t = 0; t < nt; ++t) {
+  if (t0 < nt) { fetch(t0); put(); }
+  for (int t = t0; t < nt; ++t) {
     const int j0 = tl.at(t) * BK;
     const bool more = t + 1 < nt;
     __syncthreads();
@@ -581,6 +601,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
     if (more) put();
   }
   if (!live || !a.gq) return;
+  if (a.nsplit > 1) {
+    float* po = a.part + (((int64_t)sp * (a.b * a.hk) + bh) * a.rows + row) * a.d;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int c = m * 32 + q4 * 8 + 4 * h;
+        if (c < a.d) *reinterpret_cast<f4_t*>(po + c) = f4_t{dq[m][4 * q4], dq[m][4 * q4 + 1], dq[m][4 * q4 + 2], dq[m][4 * q4 + 3]};
+      }
+    return;
+  }
   char* dp = a.gq + b * a.gqs[0] + qi * a.gqs[1] + head * a.gqs[2];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -591,6 +622,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
     }
 }
 
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bwd_q_join_kernel(AttnArgs a) {
+  const int c4 = a.d / 4;
+  const int64_t nrow = (int64_t)a.b * a.hk * a.rows, total = nrow * c4;
+  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
+    const int64_t pr = v / c4;
+    const int c = (int)(v - pr * c4) * 4, bh = (int)(pr / a.rows), row = (int)(pr - (int64_t)bh * a.rows), b = bh / a.hk;
+    const int qi = row / a.g, head = (bh - b * a.hk) * a.g + row - qi * a.g;
+    f4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < a.nsplit; ++i) s += *reinterpret_cast<const f4_t*>(a.part + (i * nrow + pr) * a.d + c);
+    T* g = (T*)(a.gq + b * a.gqs[0] + qi * a.gqs[1] + head * a.gqs[2]) + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) g[e] = (T)(s[e] * a.scale);
+  }
+}
+
 // ---- backward: dk, dv ----------------------------------------------------------------------------------------------------------------
 // A wave owns 32 keys (operands and both accumulators in registers); the workgroup's four waves walk the query tiles that may see its 128
 // keys, once for every head of the group: the gradient of a shared head is one sum in one place.  Blocks that hold sinks see every query,
@@ -599,7 +647,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
   constexpr bool kAhead = kAheadOf<T>;
-  constexpr int NW = 4, BQ = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = DP / 32;
+  constexpr int NW = 4, BQ = sizeof(T) == 2 ? 64 : 32, DL = lds_width(DP), NT = NW * 64, KS = DP / 16, MT = (DP + 31) / 32;
   using TL = Tile<T, DL>;
   __shared__ uint4 sQ[BQ * TL::CH], sG[BQ * TL::CH];
   __shared__ float sL[BQ], sD[BQ];
@@ -805,24 +853,35 @@ bool side_ok(const void* p, const int64_t* s, int es) {
     if (s[i] * es % 16) return false;
   return true;
 }
+// keys a query may see, at most: what its tiles are shared out over
+int64_t key_span(const myolo_attn_desc* d, int rows) {
+  if (!d->window) return d->lk;
+  const int64_t w = (int64_t)d->window * (d->causal ? 1 : 2) + d->sinks + rows / (d->hq / d->hk) + 128;
+  return w < d->lk ? w : d->lk;
+}
+// workgroups of 256 threads that are resident at once: two a CU, one where a kernel's registers leave a SIMD one wave
+int resident(const myolo_attn_desc* d) { return d->dtype == MYOLO_F16 || d->d <= 64 ? 512 : 256; }
 struct FwdShape { int nw, nblk, nsplit; };
 FwdShape fwd_shape(const myolo_attn_desc* d) {
   const int64_t rows = (int64_t)d->lq * (d->hq / d->hk), bh = (int64_t)d->b * d->hk;
   FwdShape f;
   f.nw = rows > 32 ? 4 : 1;
   f.nblk = (int)((rows + 32 * f.nw - 1) / (32 * f.nw));
-  // few workgroups over a long key axis: split it until there is work for four waves on every CU, a split keeping a tile at least
-  int64_t span = d->lk;
-  if (d->window) {
-    const int64_t w = (int64_t)d->window * (d->causal ? 1 : 2) + d->sinks + 32 * f.nw / (d->hq / d->hk) + 128;
-    if (w < span) span = w;
-  }
-  const int64_t tiles = (span + 63) / 64, want = 1024 / f.nw, have = bh * f.nblk;
+  // few workgroups over a long key axis: split it until every CU has four waves (single waves) or its two workgroups, a split keeping a tile
+  const int64_t tiles = (key_span(d, 32 * f.nw) + 63) / 64, want = f.nw == 1 ? 1024 : resident(d), have = bh * f.nblk;
   int64_t n = have > 0 ? want / have : 1;
   if (n > tiles) n = tiles;
   if (n > kMaxSplit) n = kMaxSplit;
   f.nsplit = n < 2 ? 1 : (int)n;
   return f;
+}
+int q_split(const myolo_attn_desc* d) {
+  const int64_t blocks = ((int64_t)d->lq * (d->hq / d->hk) + 127) / 128 * d->b * d->hk, tiles = (key_span(d, 128) + 63) / 64;
+  if (!blocks) return 1;
+  int64_t n = resident(d) / blocks;
+  if (n > tiles) n = tiles;
+  if (n > 16) n = 16;
+  return n < 2 ? 1 : (int)n;
 }
 struct KvShape { int nblk, nsb, nsplit; };
 KvShape kv_shape(const myolo_attn_desc* d) {
@@ -832,7 +891,7 @@ KvShape kv_shape(const myolo_attn_desc* d) {
   const int64_t full = (d->lq + bq - 1) / bq * g, total = bh * k.nblk;
   if (!total || !full) return k;
   int64_t n = 1;
-  const int64_t fill = d->d <= 64 ? 512 : 256;           // workgroups that are resident at once
+  const int64_t fill = d->d <= 64 && d->dtype == MYOLO_F16 ? 512 : 256;       // workgroups that are resident at once
   if (d->window && d->sinks) {
     // a block of sinks walks every query, its neighbours the band.  Cut it to the band's length where several rounds of workgroups follow it,
     // to eighths of that where the last round would wait for it (8 x 32 blocks of 128 channels: 300 -> 271 us; 64 x 16 blocks of 64: 92 -> 98)
@@ -859,7 +918,7 @@ void bytes3(int64_t* o, const int64_t* s, int64_t es) { for (int i = 0; i < 3; +
 AttnArgs args_of(const myolo_attn_desc* d) {
   const int64_t es = d->dtype == MYOLO_F16 ? 2 : 4;
   AttnArgs a{};
-  a.q = (const char*)d->q; a.k = (const char*)d->k; a.v = (const char*)d->v; a.o = (char*)d->o; a.go = (const char*)d->go;
+  a.q = (const char*)d->q; a.k = (const char*)d->k; a.v = (const char*)d->v; a.o = (char*)d->o; a.ores = d->dtype == MYOLO_F16 ? (char*)d->o_res : nullptr; a.go = (const char*)d->go;
   a.gq = (char*)d->gq; a.gk = (char*)d->gk; a.gv = (char*)d->gv;
   a.lse = d->lse; a.lens = d->lens; a.starts = d->starts;
   bytes3(a.qs, d->qs, es); bytes3(a.ks, d->ks, es); bytes3(a.vs, d->vs, es); bytes3(a.os, d->os, es);
@@ -889,15 +948,21 @@ template <typename T, int DP> int launch_fwd_w(const AttnArgs& a, int nw, hipStr
 }
 template <typename T> int run_fwd(const AttnArgs& a, int nw, hipStream_t st) {
   if (a.d <= 32) return launch_fwd_w<T, 32>(a, nw, st);
+  if (a.d <= 48) return launch_fwd_w<T, 48>(a, nw, st);
   if (a.d <= 64) return launch_fwd_w<T, 64>(a, nw, st);
+  if (a.d <= 80) return launch_fwd_w<T, 80>(a, nw, st);
   if (a.d <= 96) return launch_fwd_w<T, 96>(a, nw, st);
   return launch_fwd_w<T, 128>(a, nw, st);
 }
 template <typename T, int DP> int launch_bwd(AttnArgs& a, const KvShape& kv, hipStream_t st) {
   a.nblk = (a.rows + 127) / 128;
   if (a.rows) {
-    hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP>), dim3((unsigned)((int64_t)a.b * a.hk * a.nblk)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP>), dim3((unsigned)((int64_t)a.b * a.hk * a.nblk * a.nsplit)), dim3(256), 0, st, a);
     MYOLO_CHECK_LAUNCH();
+    if (a.nsplit > 1) {
+      hipLaunchKernelGGL((attn_bwd_q_join_kernel<T>), dim3(grid_for((int64_t)a.b * a.hk * a.rows * (a.d / 4), 256, 4096)), dim3(256), 0, st, a);
+      MYOLO_CHECK_LAUNCH();
+    }
   }
   if (a.gk && a.lk) {
     const int64_t bh = (int64_t)a.b * a.hk;
@@ -913,7 +978,9 @@ template <typename T, int DP> int launch_bwd(AttnArgs& a, const KvShape& kv, hip
 }
 template <typename T> int run_bwd(AttnArgs& a, const KvShape& kv, hipStream_t st) {
   if (a.d <= 32) return launch_bwd<T, 32>(a, kv, st);
+  if (a.d <= 48) return launch_bwd<T, 48>(a, kv, st);
   if (a.d <= 64) return launch_bwd<T, 64>(a, kv, st);
+  if (a.d <= 80) return launch_bwd<T, 80>(a, kv, st);
   if (a.d <= 96) return launch_bwd<T, 96>(a, kv, st);
   return launch_bwd<T, 128>(a, kv, st);
 }
@@ -924,7 +991,9 @@ extern "C" int64_t myolo_attn_ws_bytes(const myolo_attn_desc* d, int backward) {
   if (!desc_ok(d)) return 0;
   if (backward) {
     const KvShape k = kv_shape(d);
-    return delta_bytes(d) + (k.nsplit > 1 ? (int64_t)d->b * d->hk * k.nsb * k.nsplit * 256 * d->d * 4 : 0);
+    const int64_t kv = k.nsplit > 1 ? (int64_t)d->b * d->hk * k.nsb * k.nsplit * 256 * d->d * 4 : 0, nq = q_split(d);
+    const int64_t q = nq > 1 ? nq * d->b * d->hq * d->lq * d->d * 4 : 0;
+    return delta_bytes(d) + (q > kv ? q : kv);              // (dq's sums are joined before dk / dv's are formed)
   }
   const FwdShape f = fwd_shape(d);
   if (f.nsplit == 1) return 0;
@@ -935,6 +1004,7 @@ extern "C" int myolo_attn_fwd(const myolo_attn_desc* d, void* stream) {
   if (!desc_ok(d) || !(d->scale > 0.f)) return MYOLO_EINVAL;
   if ((int64_t)d->b * d->lq == 0) return 0;
   const int es = d->dtype == MYOLO_F16 ? 2 : 4;
+  if (d->o_res && (uintptr_t)d->o_res % 16) return MYOLO_EINVAL;
   if (!side_ok(d->q, d->qs, es) || !side_ok(d->o, d->os, es)) return MYOLO_EINVAL;
   if (d->lk && (!side_ok(d->k, d->ks, es) || !side_ok(d->v, d->vs, es))) return MYOLO_EINVAL;
   const FwdShape f = fwd_shape(d);
@@ -950,6 +1020,7 @@ extern "C" int myolo_attn_bwd(const myolo_attn_desc* d, void* stream) {
   if (!desc_ok(d) || !(d->scale > 0.f) || (d->gk == nullptr) != (d->gv == nullptr)) return MYOLO_EINVAL;
   if (d->b == 0 || (!d->gq && !d->gk)) return 0;
   const int es = d->dtype == MYOLO_F16 ? 2 : 4;
+  if (d->o_res && (uintptr_t)d->o_res % 16) return MYOLO_EINVAL;
   if (d->lq && (!side_ok(d->q, d->qs, es) || !side_ok(d->o, d->os, es) || !side_ok(d->go, d->gos, es) || !d->lse)) return MYOLO_EINVAL;
   if (d->lk && (!side_ok(d->k, d->ks, es) || !side_ok(d->v, d->vs, es))) return MYOLO_EINVAL;
   if ((d->gq && d->lq && !side_ok(d->gq, d->gqs, es)) || (d->gk && d->lk && (!side_ok(d->gk, d->gks, es) || !side_ok(d->gv, d->gvs, es))))
@@ -960,6 +1031,7 @@ extern "C" int myolo_attn_bwd(const myolo_attn_desc* d, void* stream) {
   if ((int64_t)a.b * a.hk * ((a.rows + 127) / 128) > 0x7fffffff || (int64_t)a.b * a.hk * (kv.nblk + (int64_t)kv.nsb * kv.nsplit) > 0x7fffffff) return MYOLO_EINVAL;
   a.delta = (float*)d->ws;
   a.part = (float*)((char*)d->ws + delta_bytes(d));
+  a.nsplit = d->gq ? q_split(d) : 1;
   hipStream_t st = (hipStream_t)stream;
   return d->dtype == MYOLO_F16 ? run_bwd<half_t>(a, kv, st) : run_bwd<float>(a, kv, st);
 }

@@ -283,9 +283,9 @@ Tensor side(const Tensor& t) {
   for (int i = 0; i < 3 && ok; ++i) ok = t.size(i) <= 1 || t.stride(i) * t.element_size() % 16 == 0;
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
-void attn_fill(myolo_attn_desc& d, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& lens,
-               const Tensor& starts) {
-  d.q = ptr(q); d.k = ptr(k); d.v = ptr(v); d.o = ptr(o); d.lse = (float*)ptr(lse);
+void attn_fill(myolo_attn_desc& d, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& res, const Tensor& lse,
+               const Tensor& lens, const Tensor& starts) {
+  d.q = ptr(q); d.k = ptr(k); d.v = ptr(v); d.o = ptr(o); d.o_res = ptr(res); d.lse = (float*)ptr(lse);
   d.lens = (const int*)ptr(lens); d.starts = (const int*)ptr(starts);
   strides3(d.qs, q);
   strides3(d.ks, k);
@@ -300,17 +300,17 @@ Tensor scratch(myolo_attn_desc& d, int backward, const Tensor& like) {
 }
 
 struct WindowAttentionBackward : torch::autograd::Node {
-  SavedVariable q, k, v, o, lse, lens, starts;
+  SavedVariable q, k, v, o, res, lse, lens, starts;
   myolo_attn_desc shape;                                    // sizes and options; no addresses
   variable_list apply(variable_list&& g) override {
     std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("window_attention");
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor()};
-    const Tensor Q = q.unpack(), K = k.unpack(), V = v.unpack(), O = o.unpack(shared_from_this()), S = lse.unpack(), N = lens.unpack(), P = starts.unpack();
+    const Tensor Q = q.unpack(), K = k.unpack(), V = v.unpack(), O = o.unpack(shared_from_this()), R = res.unpack(), S = lse.unpack(), N = lens.unpack(), P = starts.unpack();
     const Tensor go = side(g[0].scalar_type() == Q.scalar_type() ? g[0] : g[0].to(Q.scalar_type()));
     const bool want_q = task_should_compute_output(0), want_k = task_should_compute_output(1), want_v = task_should_compute_output(2);
     myolo_attn_desc d = shape;
-    attn_fill(d, Q, K, V, O, S, N, P);
+    attn_fill(d, Q, K, V, O, R, S, N, P);
     d.go = ptr(go);
     strides3(d.gos, go);
     Tensor gq, gk, gv;
@@ -334,7 +334,7 @@ struct WindowAttentionBackward : torch::autograd::Node {
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (SavedVariable* s : {&q, &k, &v, &o, &lse, &lens, &starts}) s->reset_data();
+    for (SavedVariable* s : {&q, &k, &v, &o, &res, &lse, &lens, &starts}) s->reset_data();
   }
   std::string name() const override { return "WindowAttentionBackward"; }
 };
@@ -358,7 +358,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
   myolo_attn_desc shape{};
   shape.b = (int32_t)b; shape.lq = (int32_t)lq; shape.lk = (int32_t)lk; shape.hq = (int32_t)hq; shape.hk = (int32_t)hk; shape.d = (int32_t)dim;
   shape.dtype = dtype_of(q); shape.causal = causal; shape.window = (int32_t)window; shape.sinks = (int32_t)std::min(sinks, lk); shape.scale = (float)scale;
-  Tensor Q, K, V, out, lse;
+  Tensor Q, K, V, out, res, lse;
   {
     at::NoGradGuard off;
     Q = side(q);
@@ -367,9 +367,12 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
     if (lens.defined()) lens = lens.contiguous();
     if (starts.defined()) starts = starts.contiguous();
     out = empty(q.sizes(), q);
-    if (train) lse = floats(b * hq * lq, q);
+    if (train) {
+      lse = floats(b * hq * lq, q);
+      if (q.scalar_type() == at::kHalf) res = empty(q.sizes(), q);
+    }
     myolo_attn_desc d = shape;
-    attn_fill(d, Q, K, V, out, lse, lens, starts);
+    attn_fill(d, Q, K, V, out, res, lse, lens, starts);
     const Tensor ws = scratch(d, 0, q);
     On on(q);
     check(lib.attn_fwd(&d, on.stream), "myolo_attn_fwd");
@@ -380,6 +383,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
     fn->q = SavedVariable(Q, false);
     fn->k = SavedVariable(K, false);
     fn->v = SavedVariable(V, false);
+    fn->res = SavedVariable(res, false);
     fn->lse = SavedVariable(lse, false);
     fn->lens = SavedVariable(lens, false);
     fn->starts = SavedVariable(starts, false);

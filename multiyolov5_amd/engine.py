@@ -1058,6 +1058,9 @@ class WindowAttnOp(Op):
         if plan.training:
             self.lse = torch.zeros(q.n * d.hq * n, dtype=torch.float32, device=plan.device)
             d.lse = self.lse.data_ptr()
+            if plan.dtype == torch.float16:
+                self.res = torch.zeros_like(self.out.buf.t)          # (o's layout: the rounding the backward puts back)
+                d.o_res = self.res.data_ptr() + self.out.coff * 2
             g = [t.desc(grad=True) for t in (self.out, self.q, self.k, self.v)]
             d.go, d.gq, d.gk, d.gv = (t.ptr for t in g)
             d.gos, d.gqs, d.gks, d.gvs = (_token_strides(t, self.dim) for t in g)

@@ -26,7 +26,7 @@ def lib():
 @pytest.mark.skipif(not shutil.which('gcc'), reason='no C compiler')
 def test_descriptor_layouts():
     fields = {'myolo_rope_desc': (L.RopeDesc, ['pos', 'axis', 'qs', 'ps', 'b', 'dtype']),
-              'myolo_attn_desc': (L.AttnDesc, ['lse', 'go', 'ws', 'ws_bytes', 'qs', 'gvs', 'b', 'sinks', 'scale'])}
+              'myolo_attn_desc': (L.AttnDesc, ['o_res', 'lse', 'go', 'ws', 'ws_bytes', 'qs', 'gvs', 'b', 'sinks', 'scale'])}
     src = '#include <stdio.h>\n#include <stddef.h>\n#include "myolo.h"\nint main(void){\n'
     want = []
     for name, (cls, fs) in fields.items():
@@ -103,7 +103,7 @@ def attn_desc(**kw):
 def test_attention_refusals(lib):
     shape = [dict(hk=3), dict(hq=0), dict(hk=0), dict(d=12), dict(d=0), dict(d=136), dict(dtype=L.U8), dict(window=-1), dict(sinks=-1), dict(lq=-1), dict(b=-1),
              dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(lk=(1 << 28) + 1), dict(window=(1 << 28) + 1), dict(lq=(1 << 28)), dict(b=1 << 23),
-             dict(q=FAKE + 2), dict(q=0), dict(o=0), dict(k=0), dict(v=FAKE + 8), dict(ks=(64 * 128, 130, 64)), dict(os=(64 * 256, 256, 63))]
+             dict(q=FAKE + 2), dict(q=0), dict(o=0), dict(k=0), dict(v=FAKE + 8), dict(ks=(64 * 128, 130, 64)), dict(os=(64 * 256, 256, 63)), dict(o_res=FAKE + 2)]
     for kw in shape:
         d = attn_desc(**kw)
         assert lib.myolo_attn_fwd(C.byref(d), None) == EINVAL, kw
