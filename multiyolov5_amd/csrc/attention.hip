@@ -334,23 +334,27 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) m2 = fmaxf(m2, s[u][r]);
-    m2 = fmaxf(mx, half_max(m2) * a.sl2);
-    const float use = m2 == -INFINITY ? 0.f : m2;
-    const float al = __builtin_amdgcn_exp2f(mx - use);
-    mx = m2;
-    float ls = 0.f;
+    // the reference maximum follows the running one only when that has outgrown it by 2^8 (in fp16 a probability may be that large): after the
+    // first tiles the sums are hardly ever rescaled
+    m2 = half_max(m2) * a.sl2;
+    if (__any(m2 > mx + 8.f)) {
+      m2 = fmaxf(mx, m2);
+      const float al = __builtin_amdgcn_exp2f(mx - (m2 == -INFINITY ? 0.f : m2));
+      mx = m2;
+      l *= al;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[m][r] *= al;
+    }
+    const float use = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.sl2, -use));
-        ls += s[u][r];
+        l += s[u][r];
       }
-    l = l * al + ls;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[m][r] *= al;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       Frag<T> p0, p1, vf;
