@@ -272,11 +272,6 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
   const int qi = (live ? row : r1) / a.g, head = kh * a.g + (live ? row : r1) - qi * a.g;
   const int p = vis.start + qi;
 
-  Frag<T> qf[KS];
-  const char* qp = a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) frag_global(qf[s], qp + (s * 16 + h * 8) * sizeof(T), live & (s * 16 + h * 8 < a.d));
-
   const char* kp = a.k + b * a.ks[0] + kh * a.ks[2];
   const char* vp = a.v + b * a.vs[0] + kh * a.vs[2];
   f16_t o[MT];
@@ -304,7 +299,13 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
     gk.template store<DL>(sK, tid);
     gv.template store<DL>(sV, tid);
   };
-  if (t0 < t1) { fetch(t0); put(); }
+  if (t0 < t1) fetch(t0);                                  // (in flight beside the query operands)
+  Frag<T> qf[KS];
+  const char* qp = a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) frag_global(qf[s], qp + (s * 16 + h * 8) * sizeof(T), live & (s * 16 + h * 8 < a.d));
+
+  if (t0 < t1) put();
   for (int t = t0; t < t1; ++t) {
     const int j0 = tl.at(t) * BK;
     const bool more = t + 1 < t1;
@@ -419,9 +420,61 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
     }
 }
 
-// joins the splits of a row: o = sum o_s 2^(m_s - M) / sum l_s 2^(m_s - M).  A workgroup per row: one wave forms the weights (a lane a split),
-// then 8 x 32 threads take every eighth split of four channels; the sums meet in LDS in a fixed order.  (One thread a channel group over all
-// splits took 12 us for 256 rows x 16 splits: a chain of loads.)
+// joins the splits of a row: o = sum o_s 2^(m_s - M) / sum l_s 2^(m_s - M)
+template <typename T> __device__ __forceinline__ void join_store(const AttnArgs& a, int64_t pr, int c, const f4_t& o, float inv) {
+  const int bh = (int)(pr / a.rows), row = (int)(pr - (int64_t)bh * a.rows), b = bh / a.hk;
+  const int qi = row / a.g, head = (bh - b * a.hk) * a.g + row - qi * a.g;
+  T* op = (T*)(a.o + b * a.os[0] + qi * a.os[1] + head * a.os[2]) + c;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float x = pin(o[e] * inv);
+    const T v = (T)x;
+    op[e] = v;
+    if (a.ores) ((T*)(a.ores + ((char*)op - a.o)))[e] = (T)(x - (float)v);
+  }
+}
+__device__ __forceinline__ void join_lse(const AttnArgs& a, int64_t pr, float mx, float sum) {
+  const int bh = (int)(pr / a.rows), row = (int)(pr - (int64_t)bh * a.rows), b = bh / a.hk;
+  const int qi = row / a.g, head = (bh - b * a.hk) * a.g + row - qi * a.g;
+  a.lse[((int64_t)b * a.hq + head) * a.lq + qi] = sum == 0.f ? -INFINITY : mx + __log2f(sum);
+}
+// few splits: a thread takes four channels of a row over all of them
+constexpr int kFewSplits = 8;
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a) {
+  const int c4 = a.d / 4;
+  const int64_t nrow = (int64_t)a.b * a.hk * a.rows, total = nrow * c4;
+  const float* ml = a.part + (int64_t)a.nsplit * nrow * a.d;
+  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
+    const int64_t pr = v / c4;
+    const int c = (int)(v - pr * c4) * 4;
+    f4_t x[kFewSplits];
+    float m[kFewSplits], l[kFewSplits], mx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < kFewSplits; ++s) {
+      const bool on = s < a.nsplit;
+      const uint4 q = ldg16(on ? (const char*)(a.part + (s * nrow + pr) * a.d + c) : zero_page());
+      x[s] = *reinterpret_cast<const f4_t*>(&q);
+      m[s] = on ? ml[(s * nrow + pr) * 2] : -INFINITY;
+      l[s] = on ? ml[(s * nrow + pr) * 2 + 1] : 0.f;
+    }
+#pragma unroll
+    for (int s = 0; s < kFewSplits; ++s) mx = fmaxf(mx, m[s]);
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kFewSplits; ++s) {
+      const float w = __builtin_amdgcn_exp2f(m[s] - (mx == -INFINITY ? 0.f : mx));
+      sum += w * l[s];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += w * x[s][e];
+    }
+    if (a.lse && c == 0) join_lse(a, pr, mx, sum);
+    join_store<T>(a, pr, c, o, sum == 0.f ? 0.f : 1.f / sum);
+  }
+}
+// many splits (one token over a long cache): a workgroup a row.  One wave forms the weights (a lane a split), then 8 x 32 threads take every
+// eighth split of four channels; the sums meet in LDS in a fixed order.  256 rows x 16 splits: 5 us, 12 with a thread over all splits;
+// 4662 rows x 4 splits: 27 us, 5 with a thread.
 constexpr int kMaxSplit = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
@@ -440,8 +493,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
       const uint4 v = ldg16(on ? (const char*)(a.part + (s * nrow + pr) * a.d + c) : zero_page());
       x[i] = *reinterpret_cast<const f4_t*>(&v);
     }
-    const int bh = (int)(pr / a.rows), row = (int)(pr - (int64_t)bh * a.rows), b = bh / a.hk;
-    const int qi = row / a.g, head = (bh - b * a.hk) * a.g + row - qi * a.g;
     if (threadIdx.x < 64) {
       const int s = threadIdx.x;
       const bool on = s < a.nsplit;
@@ -453,7 +504,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
       sw[s] = w;
       if (s == 0) {
         sinv = sum == 0.f ? 0.f : 1.f / sum;
-        if (a.lse) a.lse[((int64_t)b * a.hq + head) * a.lq + qi] = sum == 0.f ? -INFINITY : mx + __log2f(sum);
+        if (a.lse) join_lse(a, pr, mx, sum);
       }
     }
     __syncthreads();
@@ -467,14 +518,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     if (sg == 0 && c < a.d) {
 #pragma unroll
       for (int k = 1; k < 8; ++k) o += so[k][cg];
-      T* op = (T*)(a.o + b * a.os[0] + qi * a.os[1] + head * a.os[2]) + c;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = pin(o[e] * sinv);
-        const T v = (T)x;
-        op[e] = v;
-        if (a.ores) ((T*)(a.ores + ((char*)op - a.o)))[e] = (T)(x - (float)v);
-      }
+      join_store<T>(a, pr, c, o, sinv);
     }
     __syncthreads();
   }
@@ -520,8 +564,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
     frag_global(gf[s], gp + c * sizeof(T), ok);
     frag_global(of, op + c * sizeof(T), ok);
     delta += frag_dot(gf[s], of);
-    if (a.ores) {
-      frag_global(of, a.ores + (op - a.o) + c * sizeof(T), ok);
+    if constexpr (sizeof(T) == 2) {                          // (a select, not a branch: eight waits in a row cost a seventh of the kernel)
+      frag_global(of, a.ores + (op - a.o) + c * sizeof(T), ok & (a.ores != nullptr));
       delta += frag_dot(gf[s], of);
     }
   }
@@ -685,15 +729,6 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_
     t1 = min(t0 + n, t1);
   }
 
-  Frag<T> kf[KS], vf[KS];
-  const char* kp = a.k + b * a.ks[0] + kh * a.ks[2] + (int64_t)key * a.ks[1];
-  const char* vp = a.v + b * a.vs[0] + kh * a.vs[2] + (int64_t)key * a.vs[1];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int c = s * 16 + h * 8;
-    frag_global(kf[s], kp + c * sizeof(T), seen & (c < a.d));
-    frag_global(vf[s], vp + c * sizeof(T), seen & (c < a.d));
-  }
   f16_t dk[MT], dv[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) dk[m] = dv[m] = f16_t{};
@@ -718,7 +753,17 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_
     gg.template store<DL>(sG, tid);
     if (tid < BQ) { sL[tid] = nl; sD[tid] = nd; }
   };
-  if (t0 < t1) { fetch(t0); put(); }
+  if (t0 < t1) fetch(t0);                                  // (in flight beside the key operands)
+  Frag<T> kf[KS], vf[KS];
+  const char* kp = a.k + b * a.ks[0] + kh * a.ks[2] + (int64_t)key * a.ks[1];
+  const char* vp = a.v + b * a.vs[0] + kh * a.vs[2] + (int64_t)key * a.vs[1];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int c = s * 16 + h * 8;
+    frag_global(kf[s], kp + c * sizeof(T), seen & (c < a.d));
+    frag_global(vf[s], vp + c * sizeof(T), seen & (c < a.d));
+  }
+  if (t0 < t1) put();
   for (int t = t0; t < t1; ++t) {
     const int hd = t / nq, i0 = (q0 + t - hd * nq) * BQ;
     const bool more = t + 1 < t1;
@@ -940,7 +985,9 @@ int launch_fwd(const AttnArgs& a, hipStream_t st) {
   if (a.nsplit > 1) {
     hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, true>), grid, dim3(NW * 64), 0, st, a);
     MYOLO_CHECK_LAUNCH();
-    hipLaunchKernelGGL((attn_join_kernel<T>), dim3(grid_for((int64_t)a.b * a.hk * a.rows, 1, 1 << 16)), dim3(256), 0, st, a);
+    const int64_t nrow = (int64_t)a.b * a.hk * a.rows;
+    if (a.nsplit <= kFewSplits) hipLaunchKernelGGL((attn_join_few_kernel<T>), dim3(grid_for(nrow * (a.d / 4), 256, 4096)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attn_join_kernel<T>), dim3(grid_for(nrow, 1, 1 << 16)), dim3(256), 0, st, a);
   } else {
     hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NW, false>), grid, dim3(NW * 64), 0, st, a);
   }
