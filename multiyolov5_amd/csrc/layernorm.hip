@@ -385,8 +385,10 @@ __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* ws, 
   const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4;
   const int col = blockIdx.x * 16 + cl;                  // 0 .. 2c: gamma's channels, then beta's
   float s = 0.f;
-  if (col < 2 * c)
+  if (col < 2 * c) {
+#pragma unroll 8
     for (int i = sl; i < n; i += 64) s += ws[(int64_t)i * 2 * c + col];
+  }
   sm[sl][cl] = s;
   __syncthreads();
   if (sl == 0 && col < 2 * c) {

@@ -96,8 +96,9 @@ def window_attention(q, k, v, window=0, sinks=0, causal=False, lens=None, starts
     Query i stands at position p = starts[b] + i (starts None: Lk - Lq + i, the newest tokens of a sequence).  It sees key j when
     j < lens[b] (lens None: Lk), and not causal or j <= p, and window == 0 or |p - j| < window or j < sinks: the first `sinks` keys stay
     visible however far the window has moved.  lens, starts: int32 [B] on the device (a padded batch; a cache longer than what it holds).
-    A query that sees nothing gives zeros and takes no gradient.  What keys hold that no query of the call sees does not matter; a key that
-    only some of the queries see has to be finite.  scale: default D^-1/2, > 0.  One new token over a long cache is split over the key
+    A query that sees nothing gives zeros and takes no gradient.  What keys hold that no query of the call sees, and queries that see nothing,
+    does not matter; everything else has to be finite: a NaN in a key that some queries see, or in a query that sees some keys, may also reach
+    the results of its neighbours (64 tokens), as 0 * NaN does in a product of masked probabilities.  scale: default D^-1/2, > 0.  One new token over a long cache is split over the key
     axis.  Gradients for q, k and v, formed without atomics (a run repeats bit for bit)."""
     _tensor(q, 'window_attention: q', dim=4)
     _tensor(k, 'window_attention: k', q.dtype, 4)

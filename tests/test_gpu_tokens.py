@@ -92,6 +92,11 @@ def test_layer_norm_empty_and_partial_gradients():
     y = T().layer_norm(x, w)
     gx, gw = torch.autograd.grad(y, (x, w), torch.zeros_like(y))
     assert gx.shape == (0, 16) and bool((gw == 0).all())
+    v, gv = rnd(7, 40).cuda().requires_grad_(), rnd(8, 40)                   # a single row without a row dimension
+    y = T().layer_norm(v)
+    ref = R.layer_norm(v.detach().cpu()[None], None, None, 1e-5, gv[None])
+    R.within('one row', y[None], *ref['y'])
+    R.within('one row gx', torch.autograd.grad(y, v, gv.cuda())[0][None], *ref['gx'])
     x, go, w = rnd(1, 50, 24), rnd(2, 50, 24), rnd(3, 24)
     ref = R.layer_norm(x, w, None, 1e-5, go)
     xd, wd = x.cuda(), w.cuda().requires_grad_()

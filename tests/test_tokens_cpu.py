@@ -135,6 +135,16 @@ def test_rope_table():
     assert all(abs(t * 2 * math.pi - f) <= 1e-15 for t, f in zip(turns, (1.0, 0.1, 1.0, 0.1)))
 
 
+def test_autograd_nodes_load_and_raise_the_frameworks_error(lib):
+    ext = T._ext()
+    assert ext is T._ext()
+    with pytest.raises(L.MyoloError, match='no channels'):
+        ext.layer_norm(torch.zeros(3, 0), None, None, 1e-5)
+    q = torch.zeros(1, 2, 3, 16)
+    with pytest.raises(L.MyoloError, match='3 query heads over 2 key heads'):
+        ext.window_attention(q, q[:, :, :2], q[:, :, :2], 0, 0, False, None, None, None)
+
+
 def test_cpu_tensors_are_refused():
     q, pos = torch.zeros(1, 2, 2, 16), torch.zeros(2, 1, dtype=torch.int64)
     for f in (lambda: T.layer_norm(q), lambda: T.rope_axes(q, q, pos, (8,)), lambda: T.window_attention(q, q, q)):
