@@ -317,63 +317,63 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
     __syncthreads();
     if (more) fetch(t + 1);
     if (vis.any(pw0, pw1, j0, j0 + BK - 1)) {
-    f16_t s[U];
+      f16_t s[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      s[u] = f16_t{};
+      for (int u = 0; u < U; ++u) {
+        s[u] = f16_t{};
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        Frag<T> kf;
-        TL::row_frag(kf, sK, u * 32 + (lane & 31), k * 2 + h);
-        s[u] = mma(kf, qf[k], s[u]);
+        for (int k = 0; k < KS; ++k) {
+          Frag<T> kf;
+          TL::row_frag(kf, sK, u * 32 + (lane & 31), k * 2 + h);
+          s[u] = mma(kf, qf[k], s[u]);
+        }
       }
-    }
-    if (!vis.all(pw0, pw1, j0, j0 + BK - 1)) {
+      if (!vis.all(pw0, pw1, j0, j0 + BK - 1)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[u][r] = lkeys.has(j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[u][r] : -INFINITY;
+      }
+      float m2 = s[0][0];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[u][r] = lkeys.has(j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[u][r] : -INFINITY;
-    }
-    float m2 = s[0][0];
+        for (int r = 0; r < 16; ++r) m2 = fmaxf(m2, s[u][r]);
+      // the reference maximum follows the running one only when that has outgrown it by 2^8 (in fp16 a probability may be that large): after the
+      // first tiles the sums are hardly ever rescaled
+      m2 = half_max(m2) * a.sl2;
+      if (__any(m2 > mx + 8.f)) {
+        m2 = fmaxf(mx, m2);
+        const float al = __builtin_amdgcn_exp2f(mx - (m2 == -INFINITY ? 0.f : m2));
+        mx = m2;
+        l *= al;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) m2 = fmaxf(m2, s[u][r]);
-    // the reference maximum follows the running one only when that has outgrown it by 2^8 (in fp16 a probability may be that large): after the
-    // first tiles the sums are hardly ever rescaled
-    m2 = half_max(m2) * a.sl2;
-    if (__any(m2 > mx + 8.f)) {
-      m2 = fmaxf(mx, m2);
-      const float al = __builtin_amdgcn_exp2f(mx - (m2 == -INFINITY ? 0.f : m2));
-      mx = m2;
-      l *= al;
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[m][r] *= al;
-    }
-    const float use = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.sl2, -use));
-        l += s[u][r];
+          for (int r = 0; r < 16; ++r) o[m][r] *= al;
       }
+      const float use = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      Frag<T> p0, p1, vf;
-      frag_from<0>(p0, s[u]);
-      frag_from<1>(p1, s[u]);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        TL::col_frag(vf, sV, u * 32, m * 32, lane);
-        o[m] = mma(vf, p0, o[m]);
-        TL::col_frag(vf, sV, u * 32 + 16, m * 32, lane);
-        o[m] = mma(vf, p1, o[m]);
+        for (int r = 0; r < 16; ++r) {
+          s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.sl2, -use));
+          l += s[u][r];
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        Frag<T> p0, p1, vf;
+        frag_from<0>(p0, s[u]);
+        frag_from<1>(p1, s[u]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          TL::col_frag(vf, sV, u * 32, m * 32, lane);
+          o[m] = mma(vf, p0, o[m]);
+          TL::col_frag(vf, sV, u * 32 + 16, m * 32, lane);
+          o[m] = mma(vf, p1, o[m]);
+        }
       }
-    }
     }
     __syncthreads();
     if (more) put();
@@ -608,50 +608,50 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
     __syncthreads();
     if (more) fetch(t + 1);
     if (vis.any(pw0, pw1, j0, j0 + BK - 1)) {
-    const bool all = vis.all(pw0, pw1, j0, j0 + BK - 1);
+      const bool all = vis.all(pw0, pw1, j0, j0 + BK - 1);
 #pragma unroll
-    for (int u = 0; u < BK / 32; ++u) {
-      f16_t s = f16_t{}, dp = f16_t{};
-      if constexpr (kAhead) {
-        Frag<T> fk[KS], fv[KS];
+      for (int u = 0; u < BK / 32; ++u) {
+        f16_t s = f16_t{}, dp = f16_t{};
+        if constexpr (kAhead) {
+          Frag<T> fk[KS], fv[KS];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) TL::row_frag(fk[k], sK, u * 32 + (lane & 31), k * 2 + h);
+          for (int k = 0; k < KS; ++k) TL::row_frag(fk[k], sK, u * 32 + (lane & 31), k * 2 + h);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) TL::row_frag(fv[k], sV, u * 32 + (lane & 31), k * 2 + h);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int k = 0; k < KS; ++k) TL::row_frag(fv[k], sV, u * 32 + (lane & 31), k * 2 + h);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) s = mma(fk[k], qf[k], s);
+          for (int k = 0; k < KS; ++k) s = mma(fk[k], qf[k], s);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) dp = mma(fv[k], gf[k], dp);
-      } else {
+          for (int k = 0; k < KS; ++k) dp = mma(fv[k], gf[k], dp);
+        } else {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          Frag<T> f;
-          TL::row_frag(f, sK, u * 32 + (lane & 31), k * 2 + h);
-          s = mma(f, qf[k], s);
-          TL::row_frag(f, sV, u * 32 + (lane & 31), k * 2 + h);
-          dp = mma(f, gf[k], dp);
+          for (int k = 0; k < KS; ++k) {
+            Frag<T> f;
+            TL::row_frag(f, sK, u * 32 + (lane & 31), k * 2 + h);
+            s = mma(f, qf[k], s);
+            TL::row_frag(f, sV, u * 32 + (lane & 31), k * 2 + h);
+            dp = mma(f, gf[k], dp);
+          }
+        }
+        Columns<T, DL, kAhead> ck(sK, u * 32, lane);
+        ck.first();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, -lse)) * (dp[r] - delta);
+        if (!all) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = lkeys.has(j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[r] : 0.f;
+        }
+        Frag<T> d0, d1;
+        frag_from<0>(d0, s);
+        frag_from<1>(d1, s);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (m + 1 < MT) ck.next(m);
+          ck.now(m);
+          dq[m] = mma(ck.a(m), d0, dq[m]);
+          dq[m] = mma(ck.b(m), d1, dq[m]);
         }
       }
-      Columns<T, DL, kAhead> ck(sK, u * 32, lane);
-      ck.first();
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, -lse)) * (dp[r] - delta);
-      if (!all) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = lkeys.has(j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[r] : 0.f;
-      }
-      Frag<T> d0, d1;
-      frag_from<0>(d0, s);
-      frag_from<1>(d1, s);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (m + 1 < MT) ck.next(m);
-        ck.now(m);
-        dq[m] = mma(ck.a(m), d0, dq[m]);
-        dq[m] = mma(ck.b(m), d1, dq[m]);
-      }
-    }
     }
     __syncthreads();
     if (more) put();
@@ -780,73 +780,73 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_
     if (more) fetch(t + 1);
     const int p0 = vis.start + i0, p1 = p0 + BQ - 1;
     if ((kw0 <= kw1) & vis.any(p0, p1, kw0, kw1)) {
-    const bool all = kw0 + 31 < a.lk && i0 + BQ <= a.lq && vis.all(p0, p1, kw0, kw1);
+      const bool all = kw0 + 31 < a.lk && i0 + BQ <= a.lq && vis.all(p0, p1, kw0, kw1);
 #pragma unroll 1
-    for (int u = 0; u < BQ / 32; ++u) {
-      // fp16: the row operands of both products are read ahead of their matrix instructions, the column operands a step ahead, so that exp
-      // runs beside the second product and dS beside dv (fp32 operands are twice the registers and a sixteenth of the rate: read in place)
-      f16_t s = f16_t{}, dp = f16_t{};
-      if constexpr (kAhead) {
-        Frag<T> fq[KS], fg[KS];
+      for (int u = 0; u < BQ / 32; ++u) {
+        // fp16: the row operands of both products are read ahead of their matrix instructions, the column operands a step ahead, so that exp
+        // runs beside the second product and dS beside dv (fp32 operands are twice the registers and a sixteenth of the rate: read in place)
+        f16_t s = f16_t{}, dp = f16_t{};
+        if constexpr (kAhead) {
+          Frag<T> fq[KS], fg[KS];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) TL::row_frag(fq[k], sQ, u * 32 + (lane & 31), k * 2 + h);
+          for (int k = 0; k < KS; ++k) TL::row_frag(fq[k], sQ, u * 32 + (lane & 31), k * 2 + h);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) TL::row_frag(fg[k], sG, u * 32 + (lane & 31), k * 2 + h);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int k = 0; k < KS; ++k) TL::row_frag(fg[k], sG, u * 32 + (lane & 31), k * 2 + h);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) s = mma(fq[k], kf[k], s);
+          for (int k = 0; k < KS; ++k) s = mma(fq[k], kf[k], s);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) dp = mma(fg[k], vf[k], dp);
-      } else {
+          for (int k = 0; k < KS; ++k) dp = mma(fg[k], vf[k], dp);
+        } else {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          Frag<T> f;
-          TL::row_frag(f, sQ, u * 32 + (lane & 31), k * 2 + h);
-          s = mma(f, kf[k], s);
-          TL::row_frag(f, sG, u * 32 + (lane & 31), k * 2 + h);
-          dp = mma(f, vf[k], dp);
+          for (int k = 0; k < KS; ++k) {
+            Frag<T> f;
+            TL::row_frag(f, sQ, u * 32 + (lane & 31), k * 2 + h);
+            s = mma(f, kf[k], s);
+            TL::row_frag(f, sG, u * 32 + (lane & 31), k * 2 + h);
+            dp = mma(f, vf[k], dp);
+          }
+        }
+        Columns<T, DL, kAhead> cg(sG, u * 32, lane), cq(sQ, u * 32, lane);
+        cg.first();
+        f4_t l4[4], d4[4];
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          l4[r4] = *reinterpret_cast<const f4_t*>(sL + u * 32 + 8 * r4 + 4 * h);
+          d4[r4] = *reinterpret_cast<const f4_t*>(sD + u * 32 + 8 * r4 + 4 * h);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, l4[r >> 2][r & 3]));
+        if (!all) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = lrows.has(p0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[r] : 0.f;
+        }
+        Frag<T> f0, f1;
+        frag_from<0>(f0, s);
+        frag_from<1>(f1, s);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = s[r] * fmaf(dp[r], kPUnshift, -d4[r >> 2][r & 3]);
+        if (!all) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] = lrows.has(p0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? dp[r] : 0.f;
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (m + 1 < MT) cg.next(m); else cq.first();
+          cg.now(m);
+          dv[m] = mma(f0, cg.a(m), dv[m]);
+          dv[m] = mma(f1, cg.b(m), dv[m]);
+        }
+        frag_from<0>(f0, dp);
+        frag_from<1>(f1, dp);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (m + 1 < MT) cq.next(m);
+          cq.now(m);
+          dk[m] = mma(f0, cq.a(m), dk[m]);
+          dk[m] = mma(f1, cq.b(m), dk[m]);
         }
       }
-      Columns<T, DL, kAhead> cg(sG, u * 32, lane), cq(sQ, u * 32, lane);
-      cg.first();
-      f4_t l4[4], d4[4];
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        l4[r4] = *reinterpret_cast<const f4_t*>(sL + u * 32 + 8 * r4 + 4 * h);
-        d4[r4] = *reinterpret_cast<const f4_t*>(sD + u * 32 + 8 * r4 + 4 * h);
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, l4[r >> 2][r & 3]));
-      if (!all) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = lrows.has(p0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[r] : 0.f;
-      }
-      Frag<T> f0, f1;
-      frag_from<0>(f0, s);
-      frag_from<1>(f1, s);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] = s[r] * fmaf(dp[r], kPUnshift, -d4[r >> 2][r & 3]);
-      if (!all) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = lrows.has(p0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? dp[r] : 0.f;
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (m + 1 < MT) cg.next(m); else cq.first();
-        cg.now(m);
-        dv[m] = mma(f0, cg.a(m), dv[m]);
-        dv[m] = mma(f1, cg.b(m), dv[m]);
-      }
-      frag_from<0>(f0, dp);
-      frag_from<1>(f1, dp);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (m + 1 < MT) cq.next(m);
-        cq.now(m);
-        dk[m] = mma(f0, cq.a(m), dk[m]);
-        dk[m] = mma(f1, cq.b(m), dk[m]);
-      }
-    }
     }
     __syncthreads();
     if (more) put();
