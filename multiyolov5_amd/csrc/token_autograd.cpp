@@ -5,9 +5,11 @@
 // use one library.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <array>
 #include <cmath>
@@ -63,6 +65,18 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
 void first_order_only(const char* what) {
   NEED(!at::GradMode::is_enabled(), what, ": the backward pass cannot itself be recorded for a second derivative (create_graph)");
 }
+// A leaf that an eager graph on the default stream still holds has its gradient's node there: the engine would make that stream wait for the one
+// being captured, which no capture survives (the error ends the process).  Refused while the capture is still whole.
+void capturable(const torch::autograd::Node& n, const Tensor& like, const char* what) {
+  const c10::DeviceGuard guard(like.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const auto& e : n.next_edges()) {
+    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) continue;
+    const auto s = e.function->stream();
+    NEED(!s || s->id() != 0 || c10::hip::getCurrentHIPStream(like.get_device()).id() == 0, what,
+         ": backward captured while an eager graph of the same leaf lives on the default stream: drop that graph, or capture with detached leaves");
+  }
+}
 Tensor empty(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape, like.options()); }
 Tensor floats(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -113,6 +127,7 @@ struct LayerNormBackward : torch::autograd::Node {
     first_order_only("layer_norm");
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const Tensor X = x.unpack(), W = w.unpack(), S = saved.unpack();
+    capturable(*this, X, "layer_norm");
     myolo_tensor xd, gd;
     rows_of(X, xd);                                        // (saved as its rows were read: never copied again)
     Tensor go = g[0].scalar_type() == X.scalar_type() ? g[0] : g[0].to(X.scalar_type());
@@ -226,6 +241,7 @@ struct RopeBackward : torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("rope_axes");
     const bool has_k = !ks.empty();
+    capturable(*this, pos.unpack(), "rope_axes");
     if (!g[0].defined() && !(has_k && g[1].defined())) return {Tensor(), Tensor()};
     auto grad = [&](const Tensor& t, const std::vector<int64_t>& shape) {
       return !t.defined() ? at::zeros(shape, like) : t.scalar_type() == like.dtype() ? t : t.to(like);
@@ -307,6 +323,7 @@ struct WindowAttentionBackward : torch::autograd::Node {
     first_order_only("window_attention");
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const Tensor Q = q.unpack(), K = k.unpack(), V = v.unpack(), O = o.unpack(shared_from_this()), R = res.unpack(), S = lse.unpack(), N = lens.unpack(), P = starts.unpack();
+    capturable(*this, Q, "window_attention");
     const Tensor go = side(g[0].scalar_type() == Q.scalar_type() ? g[0] : g[0].to(Q.scalar_type()));
     const bool want_q = task_should_compute_output(0), want_k = task_should_compute_output(1), want_v = task_should_compute_output(2);
     myolo_attn_desc d = shape;

@@ -1,4 +1,5 @@
 """Token operators (multiyolov5_amd/utils/tokens.py) against their 64-bit definitions (tests/token_ref.py, which derives the tolerances)."""
+import gc
 import math
 
 import pytest
@@ -581,3 +582,29 @@ def test_refusals():
                   ((q.double(), k.double(), k.double()), {})):
         with pytest.raises(MyoloError):
             t.window_attention(*a, **kw)
+
+
+def test_capture_beside_an_eager_graph_of_the_same_leaf_is_refused():
+    """a leaf whose gradient node stands on the default stream cannot take part in a capture: an error while the capture is whole, nothing worse"""
+    t = T()
+    x = rnd(1, 2, 6, 2, 16).cuda().requires_grad_()
+    pos = torch.arange(6).reshape(6, 1).cuda()
+    go = rnd(2, 2, 6, 2, 16).cuda()
+    for f in (lambda: t.layer_norm(x), lambda: t.rope_axes(x, None, pos, (8,))[0], lambda: t.window_attention(x, x, x)):
+        alive = f()
+        want = torch.autograd.grad(alive, x, go, retain_graph=True)[0]
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match='eager graph of the same leaf'):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(f(), x, go)
+        assert torch.equal(torch.autograd.grad(alive, x, go)[0], want)
+        del alive
+        gc.collect()                                                # (the error's traceback held the refused graph)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):                               # no eager graph left: the same capture is taken
+            got = torch.autograd.grad(f(), x, go)[0]
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+        del got
