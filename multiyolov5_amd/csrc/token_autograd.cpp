@@ -241,12 +241,13 @@ struct RopeBackward : torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("rope_axes");
     const bool has_k = !ks.empty();
-    capturable(*this, pos.unpack(), "rope_axes");
+    const Tensor P = pos.unpack();                          // (once: a checkpoint hands every saved tensor out a single time)
+    capturable(*this, P, "rope_axes");
     if (!g[0].defined() && !(has_k && g[1].defined())) return {Tensor(), Tensor()};
     auto grad = [&](const Tensor& t, const std::vector<int64_t>& shape) {
       return !t.defined() ? at::zeros(shape, like) : t.scalar_type() == like.dtype() ? t : t.to(like);
     };
-    auto r = turn(grad(g[0], qs), has_k ? grad(g[1], ks) : Tensor(), pos.unpack(), spec, true);
+    auto r = turn(grad(g[0], qs), has_k ? grad(g[1], ks) : Tensor(), P, spec, true);
     return {task_should_compute_output(0) ? r.first : Tensor(), task_should_compute_output(1) ? r.second : Tensor()};
   }
   void release_variables() override {
