@@ -81,6 +81,13 @@ Tensor empty(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape
 Tensor floats(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor of(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+// What a node saved may come back from saved-tensor hooks in any layout (save_on_cpu: contiguous; a user's: anything), so a backward lays it out
+// again as its kernels read it; only its values, type, shape and device are taken for granted, and those are checked.
+Tensor saved_as(const Tensor& t, at::IntArrayRef shape, at::ScalarType dtype, const at::Device& device, const char* what) {
+  NEED(t.defined() && t.sizes() == shape && t.scalar_type() == dtype && t.device() == device, what, ": a tensor saved as ", dtype, " ", shape, " on ", device,
+       " came back as ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+  return t;
+}
 
 // ---- layer norm ----------------------------------------------------------------------------------------------------------------------
 // leading dimensions merged where their strides allow, padded to three; false where they do not reduce to three strides
@@ -122,14 +129,22 @@ bool same_rows(const myolo_tensor& a, const myolo_tensor& b) { return a.n == b.n
 
 struct LayerNormBackward : torch::autograd::Node {
   SavedVariable x, w, saved;
+  std::vector<int64_t> shape;
+  at::TensorOptions like;
+  bool has_w;
   variable_list apply(variable_list&& g) override {
     std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("layer_norm");
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor()};
-    const Tensor X = x.unpack(), W = w.unpack(), S = saved.unpack();
-    capturable(*this, X, "layer_norm");
+    const int64_t c = shape.back();
+    const auto dtype = like.dtype().toScalarType();
+    const at::Device device = like.device();
+    const Tensor raw = saved_as(x.unpack(), shape, dtype, device, "layer_norm");
+    const Tensor W = has_w ? saved_as(w.unpack(), {c}, at::kFloat, device, "layer_norm").contiguous() : Tensor();
+    const Tensor S = saved_as(saved.unpack(), {2 * (raw.numel() / c)}, at::kFloat, device, "layer_norm").contiguous();
+    capturable(*this, raw, "layer_norm");
     myolo_tensor xd, gd;
-    rows_of(X, xd);                                        // (saved as its rows were read: never copied again)
+    const Tensor X = rows_of(raw, xd);
     Tensor go = g[0].scalar_type() == X.scalar_type() ? g[0] : g[0].to(X.scalar_type());
     go = rows_of(go, gd);
     if (!same_rows(gd, xd)) {
@@ -184,8 +199,11 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w_, const OptTensor& b_, dou
   if (train) {
     std::shared_ptr<LayerNormBackward> fn(new LayerNormBackward(), torch::autograd::deleteNode);
     fn->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
+    fn->shape = x.sizes().vec();
+    fn->like = x.options();
+    fn->has_w = W.defined();
     fn->x = SavedVariable(X, false);
-    fn->w = SavedVariable(W, false);
+    if (W.defined()) fn->w = SavedVariable(W, false);
     fn->saved = SavedVariable(saved, false);
     torch::autograd::set_history(out, fn);
   }
@@ -235,13 +253,13 @@ std::pair<Tensor, Tensor> turn(Tensor q, Tensor k, const Tensor& pos, const Rope
 struct RopeBackward : torch::autograd::Node {
   SavedVariable pos;
   RopeSpec spec;
-  std::vector<int64_t> qs, ks;
+  std::vector<int64_t> qs, ks, ps;
   at::TensorOptions like;
   variable_list apply(variable_list&& g) override {
     std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("rope_axes");
     const bool has_k = !ks.empty();
-    const Tensor P = pos.unpack();                          // (once: a checkpoint hands every saved tensor out a single time)
+    const Tensor P = saved_as(pos.unpack(), ps, at::kLong, like.device(), "rope_axes");     // (once: a checkpoint hands every saved tensor out a single time)
     capturable(*this, P, "rope_axes");
     if (!g[0].defined() && !(has_k && g[1].defined())) return {Tensor(), Tensor()};
     auto grad = [&](const Tensor& t, const std::vector<int64_t>& shape) {
@@ -285,6 +303,7 @@ std::pair<Tensor, OptTensor> rope_axes(const Tensor& q, const OptTensor& k_, con
     fn->pos = SavedVariable(pos, false);
     fn->spec = s;
     fn->qs = q.sizes().vec();
+    fn->ps = pos.sizes().vec();
     if (k.defined()) fn->ks = k.sizes().vec();
     fn->like = q.options();
     if (k.defined()) torch::autograd::set_history(variable_list{r.first, r.second}, fn);
@@ -319,11 +338,23 @@ Tensor scratch(myolo_attn_desc& d, int backward, const Tensor& like) {
 struct WindowAttentionBackward : torch::autograd::Node {
   SavedVariable q, k, v, o, res, lse, lens, starts;
   myolo_attn_desc shape;                                    // sizes and options; no addresses
+  at::TensorOptions like;
+  bool has_lens, has_starts;
   variable_list apply(variable_list&& g) override {
     std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("window_attention");
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor()};
-    const Tensor Q = q.unpack(), K = k.unpack(), V = v.unpack(), O = o.unpack(shared_from_this()), R = res.unpack(), S = lse.unpack(), N = lens.unpack(), P = starts.unpack();
+    const auto dtype = like.dtype().toScalarType();
+    const at::Device device = like.device();
+    const int64_t b = shape.b, lq = shape.lq, lk = shape.lk, hq = shape.hq, hk = shape.hk, dim = shape.d;
+    auto back = [&](const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) { return saved_as(t, sizes, type, device, "window_attention"); };
+    const Tensor Q = side(back(q.unpack(), {b, lq, hq, dim}, dtype)), K = side(back(k.unpack(), {b, lk, hk, dim}, dtype)),
+                 V = side(back(v.unpack(), {b, lk, hk, dim}, dtype));
+    // (the residual is addressed by o's strides: both dense, as the forward wrote them)
+    const Tensor O = side(back(o.unpack(shared_from_this()), {b, lq, hq, dim}, dtype).contiguous());
+    const Tensor R = dtype == at::kHalf ? side(back(res.unpack(), {b, lq, hq, dim}, dtype).contiguous()) : Tensor();
+    const Tensor S = back(lse.unpack(), {b * hq * lq}, at::kFloat).contiguous();
+    const Tensor N = has_lens ? back(lens.unpack(), {b}, at::kInt).contiguous() : Tensor(), P = has_starts ? back(starts.unpack(), {b}, at::kInt).contiguous() : Tensor();
     capturable(*this, Q, "window_attention");
     const Tensor go = side(g[0].scalar_type() == Q.scalar_type() ? g[0] : g[0].to(Q.scalar_type()));
     const bool want_q = task_should_compute_output(0), want_k = task_should_compute_output(1), want_v = task_should_compute_output(2);
@@ -401,11 +432,12 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
     fn->q = SavedVariable(Q, false);
     fn->k = SavedVariable(K, false);
     fn->v = SavedVariable(V, false);
-    fn->res = SavedVariable(res, false);
+    if (res.defined()) fn->res = SavedVariable(res, false);
     fn->lse = SavedVariable(lse, false);
-    fn->lens = SavedVariable(lens, false);
-    fn->starts = SavedVariable(starts, false);
+    if ((fn->has_lens = lens.defined())) fn->lens = SavedVariable(lens, false);
+    if ((fn->has_starts = starts.defined())) fn->starts = SavedVariable(starts, false);
     fn->shape = shape;
+    fn->like = q.options();
     torch::autograd::set_history(out, fn);
     fn->o = SavedVariable(out, true);
   }

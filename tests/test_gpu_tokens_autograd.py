@@ -14,6 +14,76 @@ DTS = pytest.mark.parametrize('dt', [F16, F32], ids=['fp16', 'fp32'])
 
 
 # ---- saved-tensor hooks ----------------------------------------------------------------------------------------------------------------
+def transposed(t):
+    """the same values, the last two axes swapped in memory: channels that are not adjacent"""
+    return t.transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() > 1 else torch.stack([t, t], -1)[..., 0]
+
+
+def shifted(t):
+    """the same values, rows off a 16-byte boundary"""
+    b = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    return b[1:].view(t.shape).copy_(t)
+
+
+def heads_first(t):
+    return t.transpose(1, 2).contiguous().transpose(1, 2) if t.dim() == 4 else t.clone()
+
+
+class every_other:
+    """another layout for every second tensor: what was laid out alike no longer is"""
+
+    def __init__(self):
+        self.n = 0
+
+    def __call__(self, t):
+        self.n += 1
+        return heads_first(t) if self.n % 2 else transposed(t)
+
+
+HOOKS = {'transposed': lambda: saved_tensors_hooks(lambda t: t.clone(), transposed), 'shifted': lambda: saved_tensors_hooks(lambda t: t.clone(), shifted),
+         'heads first': lambda: saved_tensors_hooks(lambda t: t.clone(), heads_first), 'mixed': lambda: saved_tensors_hooks(lambda t: t.clone(), every_other()),
+         'on the host': save_on_cpu, 'pinned': lambda: save_on_cpu(pin_memory=True)}
+
+
+@DTS
+@pytest.mark.parametrize('hook', list(HOOKS))
+def test_saved_tensors_in_another_layout(hook, dt):
+    x, go, w, b = rnd(1, 67, 48, dt=dt), rnd(2, 48, dt=dt).expand(67, 48), rnd(3, 48, shift=1.0), rnd(4, 48)
+    ref = R.layer_norm(x, w, b, 1e-5, go)
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    with HOOKS[hook]():
+        y = T().layer_norm(*leaves)
+    for n, t in zip(('gx', 'gw', 'gb'), torch.autograd.grad(y, leaves, go[0].cuda().expand(67, 48))):   # (a broadcast gradient is copied in the backward)
+        R.within(n, t, *ref[n])
+    q, k, v, go = rnd(1, 2, 70, 4, 32, dt=dt), rnd(2, 2, 90, 2, 32, dt=dt), rnd(3, 2, 90, 2, 32, dt=dt), rnd(4, 2, 70, 4, 32, dt=dt)
+    lens, starts = torch.tensor([90, 71], dtype=torch.int32), torch.tensor([20, 1], dtype=torch.int32)
+    kw = dict(window=23, sinks=2, causal=True)
+    ref = R.attention(q, k, v, go=go, lens=lens, starts=starts, **kw)
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    with HOOKS[hook]():
+        o = T().window_attention(*leaves, lens=lens.cuda(), starts=starts.cuda(), **kw)
+    for n, t in zip(('gq', 'gk', 'gv'), torch.autograd.grad(o, leaves, go.cuda())):
+        R.within(n, t, *ref[n])
+    pos = torch.randint(0, 90, (2, 70, 2), generator=torch.Generator().manual_seed(3))
+    leaf = q.cuda().requires_grad_()
+    with HOOKS[hook]():
+        a, _ = T().rope_axes(leaf, None, pos.cuda(), (8, 8))
+    R.within('rope', torch.autograd.grad(a, leaf, go.cuda())[0], *R.rope(go, pos, (8, 8), 10000.0, False, 'shared', True))
+
+
+@pytest.mark.parametrize('change', ['dtype', 'shape', 'device'])
+def test_saved_tensors_that_come_back_as_something_else_are_refused(change):
+    to = {'dtype': lambda t: t.double(), 'shape': lambda t: t[:1], 'device': lambda t: t.cpu()}[change]
+    x, w = rnd(1, 2, 6, 4, 16).cuda().requires_grad_(), torch.ones(16, device='cuda', requires_grad=True)
+    pos = torch.arange(12).reshape(2, 6, 1).cuda()
+    i = torch.tensor([6, 6], dtype=torch.int32, device='cuda')
+    for f in (lambda: T().layer_norm(x, w), lambda: T().window_attention(x, x, x, lens=i), lambda: T().rope_axes(x, None, pos, (8,))[0]):
+        with saved_tensors_hooks(lambda t: t, to):
+            y = f()
+        with pytest.raises(RuntimeError, match='came back as'):
+            torch.autograd.grad(y, x, torch.ones_like(y))
+
+
 def test_an_error_in_a_hook_arrives_as_itself():
     def bad(t):
         raise KeyError('mine')
