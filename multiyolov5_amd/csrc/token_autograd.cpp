@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -61,6 +62,12 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+// the kernels form no tangents: a result without one would pass for a constant downstream
+void no_forward_mode(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    NEED(!t->defined() || !t->_fw_grad(0).defined(), what, ": no derivatives in forward mode (a dual tensor)");
 }
 void first_order_only(const char* what) {
   NEED(!at::GradMode::is_enabled(), what, ": the backward pass cannot itself be recorded for a second derivative (create_graph)");
@@ -136,6 +143,7 @@ struct LayerNormBackward : torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("layer_norm");
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor()};
+    no_forward_mode("layer_norm", {&g[0]});
     const int64_t c = shape.back();
     const auto dtype = like.dtype().toScalarType();
     const at::Device device = like.device();
@@ -182,6 +190,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w_, const OptTensor& b_, dou
     NEED(!p->defined() || (p->scalar_type() == at::kFloat && p->dim() == 1 && p->size(0) == x.size(-1) && p->is_cuda()),
          "layer_norm: weight and bias are fp32 tensors of ", x.size(-1), " values on the GPU, got ", p->scalar_type(), " ", p->sizes());
   same_device(x, {&w, &b});
+  no_forward_mode("layer_norm", {&x, &w, &b});
   const bool train = wants_grad({&x, &w, &b});
   Tensor X, out, saved, W, B;
   {
@@ -259,6 +268,7 @@ struct RopeBackward : torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("rope_axes");
     const bool has_k = !ks.empty();
+    for (const Tensor& t : g) no_forward_mode("rope_axes", {&t});
     const Tensor P = saved_as(pos.unpack(), ps, at::kLong, like.device(), "rope_axes");     // (once: a checkpoint hands every saved tensor out a single time)
     capturable(*this, P, "rope_axes");
     if (!g[0].defined() && !(has_k && g[1].defined())) return {Tensor(), Tensor()};
@@ -288,6 +298,7 @@ std::pair<Tensor, OptTensor> rope_axes(const Tensor& q, const OptTensor& k_, con
            (pos.dim() == 2 || pos.size(0) == 1 || pos.size(0) == q.size(0)),
        "rope_axes: pos ", pos.sizes(), " for ", q.size(1), " tokens, ", naxis, " axes and a batch of ", q.size(0));
   same_device(q, {&k, &pos});
+  no_forward_mode("rope_axes", {&q, &k});
   RopeSpec s;
   s.npair = npair; s.naxis = naxis; s.interleaved = interleaved;
   std::copy_n(reinterpret_cast<const double*>(turns), npair, s.turns.begin());
@@ -344,6 +355,7 @@ struct WindowAttentionBackward : torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("window_attention");
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor()};
+    no_forward_mode("window_attention", {&g[0]});
     const auto dtype = like.dtype().toScalarType();
     const at::Device device = like.device();
     const int64_t b = shape.b, lq = shape.lq, lk = shape.lk, hq = shape.hq, hk = shape.hk, dim = shape.d;
@@ -403,6 +415,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
     NEED(!t->defined() || (t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == b && t->is_cuda()),
          "window_attention: lens and starts are int32 tensors of ", b, " values on the GPU, got ", t->scalar_type(), " ", t->sizes());
   same_device(q, {&k, &v, &lens, &starts});
+  no_forward_mode("window_attention", {&q, &k, &v});
   const bool train = wants_grad({&q, &k, &v});
   myolo_attn_desc shape{};
   shape.b = (int32_t)b; shape.lq = (int32_t)lq; shape.lk = (int32_t)lk; shape.hq = (int32_t)hq; shape.hk = (int32_t)hk; shape.d = (int32_t)dim;

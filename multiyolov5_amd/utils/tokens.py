@@ -5,7 +5,8 @@ The arithmetic is in libmyolo (csrc/layernorm.hip, csrc/rope.hip, csrc/attention
 host C++ over its C ABI (csrc/token_autograd.cpp): a pass over small tensors is bound by the host.  fp16 and fp32 tensors; statistics, sums
 and parameters in fp32.  Every call works on the current stream of the tensors' device, allocates its results and scratch with torch's
 allocator and never synchronises, so all of them can be captured into a graph (a backward pass not while an eager graph of the same leaves lives
-on the default stream: refused).  First derivatives only.  There is no CPU path.
+on the default stream: refused).  First derivatives in reverse mode only (second
+derivatives and dual tensors are refused).  There is no CPU path.
 """
 import ctypes as C
 import functools

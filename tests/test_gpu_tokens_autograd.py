@@ -110,3 +110,24 @@ def test_checkpointed_layer(reentrant):
     o = checkpoint(lambda *a: _layer(*a, posd, kw, *dims), *dl, use_reentrant=reentrant)
     o.backward(go.cuda())
     assert all(torch.equal(t.grad, r) for t, r in zip(dl, want))
+
+
+# ---- forward mode, tracing -------------------------------------------------------------------------------------------------------------
+def one_input(t, x, w, pos):
+    """the operators as functions of one tensor, by the argument it is"""
+    return {'layer_norm': lambda x: t.layer_norm(x, w), 'weight': lambda x: t.layer_norm(x, x[0, 0, 0]), 'rope_axes': lambda x: t.rope_axes(x, None, pos, (8,))[0],
+            'k': lambda x: t.rope_axes(x.detach(), x, pos, (8,))[1], 'window_attention': lambda x: t.window_attention(x, x.detach(), x.detach()),
+            'v': lambda x: t.window_attention(x.detach(), x.detach(), x)}
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+    x, w, pos = rnd(1, 2, 6, 4, 16).cuda(), torch.ones(16, device='cuda'), torch.arange(6).reshape(6, 1).cuda()
+    for name, f in one_input(T(), x, w, pos).items():
+        with fw.dual_level():
+            with pytest.raises(RuntimeError, match='forward mode'):
+                f(fw.make_dual(x, torch.ones_like(x)))
+            leaf = x.clone().requires_grad_()
+            y = f(leaf)                                                  # (none of it sticks)
+            with pytest.raises(RuntimeError, match='forward mode'):
+                torch.autograd.grad(y, leaf, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
