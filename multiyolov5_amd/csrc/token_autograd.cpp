@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -69,6 +70,8 @@ void no_forward_mode(const char* what, std::initializer_list<const Tensor*> ts) 
   for (const Tensor* t : ts)
     NEED(!t->defined() || !t->_fw_grad(0).defined(), what, ": no derivatives in forward mode (a dual tensor)");
 }
+// torch.jit.trace records torch's own calls: the results' empty() without the launches that fill them
+void not_traced(const char* what) { NEED(!torch::jit::tracer::isTracing(), what, ": a call cannot be traced (its kernels would be missing from the trace)"); }
 void first_order_only(const char* what) {
   NEED(!at::GradMode::is_enabled(), what, ": the backward pass cannot itself be recorded for a second derivative (create_graph)");
 }
@@ -184,6 +187,7 @@ struct LayerNormBackward : torch::autograd::Node {
 
 Tensor layer_norm(const Tensor& x, const OptTensor& w_, const OptTensor& b_, double eps) {
   const Tensor w = of(w_), b = of(b_);
+  not_traced("layer_norm");
   NEED(x.dim() > 0 && x.size(-1) >= 1 && x.size(-1) < (int64_t(1) << 31), "layer_norm: no channels in a tensor of shape ", x.sizes());
   NEED(eps >= 0.0 && std::isfinite(eps), "layer_norm: eps must be a number >= 0, got ", eps);
   for (const Tensor* p : {&w, &b})
@@ -289,6 +293,7 @@ struct RopeBackward : torch::autograd::Node {
 std::pair<Tensor, OptTensor> rope_axes(const Tensor& q, const OptTensor& k_, const Tensor& pos, int64_t turns, int64_t axis, int npair, int naxis,
                                        bool interleaved) {
   const Tensor k = of(k_);
+  not_traced("rope_axes");
   NEED(!k.defined() || (k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3) && k.size(2) >= 1),
        "rope_axes: q ", q.sizes(), " and k ", k.sizes(), " differ in more than their heads");
   NEED(q.size(2) >= 1 && q.size(3) >= 1, "rope_axes: q ", q.sizes());
@@ -403,6 +408,7 @@ struct WindowAttentionBackward : torch::autograd::Node {
 Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, bool causal, const OptTensor& lens_,
                         const OptTensor& starts_, std::optional<double> scale_) {
   Tensor lens = of(lens_), starts = of(starts_);
+  not_traced("window_attention");
   const int64_t b = q.size(0), lq = q.size(1), hq = q.size(2), dim = q.size(3), lk = k.size(1), hk = k.size(2);
   NEED(k.sizes() == v.sizes() && k.size(0) == b && k.size(3) == dim, "window_attention: q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes());
   NEED(hk >= 1 && hq >= 1 && hq % hk == 0, "window_attention: ", hq, " query heads over ", hk, " key heads");

@@ -6,7 +6,7 @@ host C++ over its C ABI (csrc/token_autograd.cpp): a pass over small tensors is 
 and parameters in fp32.  Every call works on the current stream of the tensors' device, allocates its results and scratch with torch's
 allocator and never synchronises, so all of them can be captured into a graph (a backward pass not while an eager graph of the same leaves lives
 on the default stream: refused).  First derivatives in reverse mode only (second
-derivatives and dual tensors are refused).  There is no CPU path.
+derivatives, dual tensors and calls inside torch.jit.trace are refused).  There is no CPU path.
 """
 import ctypes as C
 import functools

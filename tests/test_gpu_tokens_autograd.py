@@ -131,3 +131,11 @@ def test_forward_mode_is_refused():
             y = f(leaf)                                                  # (none of it sticks)
             with pytest.raises(RuntimeError, match='forward mode'):
                 torch.autograd.grad(y, leaf, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def test_tracing_is_refused():
+    x, w, pos = rnd(1, 2, 6, 4, 16).cuda(), torch.ones(16, device='cuda'), torch.arange(6).reshape(6, 1).cuda()
+    for name, f in one_input(T(), x, w, pos).items():
+        with pytest.raises(RuntimeError, match='traced'):
+            torch.jit.trace(f, x, check_trace=False)
+        f(x)

@@ -33,3 +33,9 @@ def test_dual_tensors_are_refused(calls, name):
     with fw.dual_level():
         with pytest.raises(L.MyoloError, match='forward mode'):
             calls[name](fw.make_dual(torch.zeros(2, 6, 4, 16), torch.ones(2, 6, 4, 16)))
+
+
+@NAMES
+def test_traced_calls_are_refused(calls, name):
+    with pytest.raises(L.MyoloError, match='traced'):
+        torch.jit.trace(calls[name], torch.zeros(2, 6, 4, 16), check_trace=False)
