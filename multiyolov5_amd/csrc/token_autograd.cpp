@@ -91,12 +91,18 @@ Tensor empty(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape
 Tensor floats(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor of(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+// t with its values in its memory: a lazily negated view (the imaginary part of a conjugate) is written out, a tensor without memory refused
+Tensor plain(const Tensor& t, const char* what) {
+  if (!t.defined()) return t;
+  NEED(!t._is_zerotensor(), what, ": a tensor without storage");
+  return t.is_neg() ? t.resolve_neg() : t;
+}
 // What a node saved may come back from saved-tensor hooks in any layout (save_on_cpu: contiguous; a user's: anything), so a backward lays it out
 // again as its kernels read it; only its values, type, shape and device are taken for granted, and those are checked.
 Tensor saved_as(const Tensor& t, at::IntArrayRef shape, at::ScalarType dtype, const at::Device& device, const char* what) {
   NEED(t.defined() && t.sizes() == shape && t.scalar_type() == dtype && t.device() == device, what, ": a tensor saved as ", dtype, " ", shape, " on ", device,
        " came back as ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
-  return t;
+  return plain(t, what);
 }
 
 // ---- layer norm ----------------------------------------------------------------------------------------------------------------------
@@ -156,7 +162,8 @@ struct LayerNormBackward : torch::autograd::Node {
     capturable(*this, raw, "layer_norm");
     myolo_tensor xd, gd;
     const Tensor X = rows_of(raw, xd);
-    Tensor go = g[0].scalar_type() == X.scalar_type() ? g[0] : g[0].to(X.scalar_type());
+    Tensor go = plain(g[0], "layer_norm");
+    if (go.scalar_type() != X.scalar_type()) go = go.to(X.scalar_type());
     go = rows_of(go, gd);
     if (!same_rows(gd, xd)) {
       go = go.contiguous();
@@ -185,9 +192,9 @@ struct LayerNormBackward : torch::autograd::Node {
   std::string name() const override { return "LayerNormBackward"; }
 };
 
-Tensor layer_norm(const Tensor& x, const OptTensor& w_, const OptTensor& b_, double eps) {
-  const Tensor w = of(w_), b = of(b_);
+Tensor layer_norm(const Tensor& x_, const OptTensor& w_, const OptTensor& b_, double eps) {
   not_traced("layer_norm");
+  const Tensor x = plain(x_, "layer_norm"), w = plain(of(w_), "layer_norm"), b = plain(of(b_), "layer_norm");
   NEED(x.dim() > 0 && x.size(-1) >= 1 && x.size(-1) < (int64_t(1) << 31), "layer_norm: no channels in a tensor of shape ", x.sizes());
   NEED(eps >= 0.0 && std::isfinite(eps), "layer_norm: eps must be a number >= 0, got ", eps);
   for (const Tensor* p : {&w, &b})
@@ -276,7 +283,8 @@ struct RopeBackward : torch::autograd::Node {
     const Tensor P = saved_as(pos.unpack(), ps, at::kLong, like.device(), "rope_axes");     // (once: a checkpoint hands every saved tensor out a single time)
     capturable(*this, P, "rope_axes");
     if (!g[0].defined() && !(has_k && g[1].defined())) return {Tensor(), Tensor()};
-    auto grad = [&](const Tensor& t, const std::vector<int64_t>& shape) {
+    auto grad = [&](const Tensor& t_, const std::vector<int64_t>& shape) {
+      const Tensor t = plain(t_, "rope_axes");
       return !t.defined() ? at::zeros(shape, like) : t.scalar_type() == like.dtype() ? t : t.to(like);
     };
     auto r = turn(grad(g[0], qs), has_k ? grad(g[1], ks) : Tensor(), P, spec, true);
@@ -290,10 +298,10 @@ struct RopeBackward : torch::autograd::Node {
 };
 
 // turns, axis: addresses of sum(sections) values each
-std::pair<Tensor, OptTensor> rope_axes(const Tensor& q, const OptTensor& k_, const Tensor& pos, int64_t turns, int64_t axis, int npair, int naxis,
+std::pair<Tensor, OptTensor> rope_axes(const Tensor& q_, const OptTensor& k_, const Tensor& pos_, int64_t turns, int64_t axis, int npair, int naxis,
                                        bool interleaved) {
-  const Tensor k = of(k_);
   not_traced("rope_axes");
+  const Tensor q = plain(q_, "rope_axes"), k = plain(of(k_), "rope_axes"), pos = plain(pos_, "rope_axes");
   NEED(!k.defined() || (k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3) && k.size(2) >= 1),
        "rope_axes: q ", q.sizes(), " and k ", k.sizes(), " differ in more than their heads");
   NEED(q.size(2) >= 1 && q.size(3) >= 1, "rope_axes: q ", q.sizes());
@@ -373,7 +381,8 @@ struct WindowAttentionBackward : torch::autograd::Node {
     const Tensor S = back(lse.unpack(), {b * hq * lq}, at::kFloat).contiguous();
     const Tensor N = has_lens ? back(lens.unpack(), {b}, at::kInt).contiguous() : Tensor(), P = has_starts ? back(starts.unpack(), {b}, at::kInt).contiguous() : Tensor();
     capturable(*this, Q, "window_attention");
-    const Tensor go = side(g[0].scalar_type() == Q.scalar_type() ? g[0] : g[0].to(Q.scalar_type()));
+    Tensor go = plain(g[0], "window_attention");
+    go = side(go.scalar_type() == Q.scalar_type() ? go : go.to(Q.scalar_type()));
     const bool want_q = task_should_compute_output(0), want_k = task_should_compute_output(1), want_v = task_should_compute_output(2);
     myolo_attn_desc d = shape;
     attn_fill(d, Q, K, V, O, R, S, N, P);
@@ -405,10 +414,11 @@ struct WindowAttentionBackward : torch::autograd::Node {
   std::string name() const override { return "WindowAttentionBackward"; }
 };
 
-Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, bool causal, const OptTensor& lens_,
+Tensor window_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window, int64_t sinks, bool causal, const OptTensor& lens_,
                         const OptTensor& starts_, std::optional<double> scale_) {
-  Tensor lens = of(lens_), starts = of(starts_);
   not_traced("window_attention");
+  const Tensor q = plain(q_, "window_attention"), k = plain(k_, "window_attention"), v = plain(v_, "window_attention");
+  Tensor lens = plain(of(lens_), "window_attention"), starts = plain(of(starts_), "window_attention");
   const int64_t b = q.size(0), lq = q.size(1), hq = q.size(2), dim = q.size(3), lk = k.size(1), hk = k.size(2);
   NEED(k.sizes() == v.sizes() && k.size(0) == b && k.size(3) == dim, "window_attention: q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes());
   NEED(hk >= 1 && hq >= 1 && hq % hk == 0, "window_attention: ", hq, " query heads over ", hk, " key heads");

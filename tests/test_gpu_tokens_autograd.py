@@ -112,6 +112,43 @@ def test_checkpointed_layer(reentrant):
     assert all(torch.equal(t.grad, r) for t, r in zip(dl, want))
 
 
+# ---- lazily negated tensors, tensors without storage -----------------------------------------------------------------------------------
+@DTS
+def test_negated_views_are_read_as_their_values(dt):
+    """(the imaginary part of a conjugate is such a view)"""
+    t, neg = T(), torch._neg_view
+    x, w, b = rnd(1, 2, 9, 4, 16, dt=dt).cuda(), rnd(2, 16).cuda(), rnd(3, 16).cuda()
+    pos = torch.arange(9).reshape(9, 1).cuda()
+    n = neg(x)
+    assert n.is_neg() and torch.equal(n, -x)
+    assert torch.equal(t.layer_norm(n, neg(w), neg(b)), t.layer_norm(-x, -w, -b))
+    assert all(torch.equal(a, r) for a, r in zip(t.rope_axes(n, n, neg(pos), (8,)), t.rope_axes(-x, -x, -pos, (8,))))
+    assert torch.equal(t.window_attention(n, x, x), t.window_attention(-x, x, x))
+    assert torch.equal(t.window_attention(x, n, x), t.window_attention(x, -x, x)) and torch.equal(t.window_attention(x, x, n), t.window_attention(x, x, -x))
+    # (one place a leaf: the engine adds the gradients of several in another order behind another graph)
+    c = x.clone()
+    for f in (lambda x: t.layer_norm(x), lambda x: t.rope_axes(x, None, pos, (8,))[0], lambda x: t.window_attention(x, c, c),
+              lambda x: t.window_attention(c, x, c), lambda x: t.window_attention(c, c, x)):
+        leaf = x.clone().requires_grad_()
+        want, = torch.autograd.grad(f(leaf), leaf, -x)
+        got, = torch.autograd.grad(f(leaf), leaf, n)                     # an incoming gradient that is negated lazily
+        assert torch.equal(got, want)
+        want, = torch.autograd.grad(f(-leaf), leaf, x)
+        got, = torch.autograd.grad(f(neg(leaf)), leaf, x)
+        assert torch.equal(got, want)
+
+
+def test_tensors_without_storage_are_refused():
+    from multiyolov5_amd._lib import MyoloError
+    t = T()
+    x, z = torch.ones(2, 6, 4, 16, device='cuda'), torch._efficientzerotensor((2, 6, 4, 16), device='cuda')
+    pos = torch.arange(6).reshape(6, 1).cuda()
+    for f in (lambda: t.layer_norm(z), lambda: t.layer_norm(x, torch._efficientzerotensor((16,), device='cuda')), lambda: t.rope_axes(z, None, pos, (8,)),
+              lambda: t.window_attention(x, z, x), lambda: t.window_attention(z, x, x)):
+        with pytest.raises(MyoloError, match='storage'):
+            f()
+
+
 # ---- forward mode, tracing -------------------------------------------------------------------------------------------------------------
 def one_input(t, x, w, pos):
     """the operators as functions of one tensor, by the argument it is"""

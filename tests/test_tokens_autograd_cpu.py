@@ -39,3 +39,9 @@ def test_dual_tensors_are_refused(calls, name):
 def test_traced_calls_are_refused(calls, name):
     with pytest.raises(L.MyoloError, match='traced'):
         torch.jit.trace(calls[name], torch.zeros(2, 6, 4, 16), check_trace=False)
+
+
+@NAMES
+def test_tensors_without_storage_are_refused(calls, name):
+    with pytest.raises(L.MyoloError, match='without storage'):
+        calls[name](torch._efficientzerotensor((2, 6, 4, 16)))
