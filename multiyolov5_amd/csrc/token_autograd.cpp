@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/AutogradState.h>
@@ -17,6 +18,7 @@
 #include <cmath>
 #include <map>
 #include <sstream>
+#include <unordered_set>
 #include "../../include/myolo.h"
 
 namespace {
@@ -76,15 +78,40 @@ void first_order_only(const char* what) {
   NEED(!at::GradMode::is_enabled(), what, ": the backward pass cannot itself be recorded for a second derivative (create_graph)");
 }
 // A leaf that an eager graph on the default stream still holds has its gradient's node there: the engine would make that stream wait for the one
-// being captured, which no capture survives (the error ends the process).  Refused while the capture is still whole.
+// being captured, which no capture survives (the error ends the process).  Refused while the capture is still whole: the node's own edges, and
+// whatever this pass is going to run behind them (a leaf under a projection, a part of the graph recorded before the capture).
 void capturable(const torch::autograd::Node& n, const Tensor& like, const char* what) {
+  using torch::autograd::Node;
   const c10::DeviceGuard guard(like.device());
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  for (const auto& e : n.next_edges()) {
-    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) continue;
-    const auto s = e.function->stream();
-    NEED(!s || s->id() != 0 || c10::hip::getCurrentHIPStream(like.get_device()).id() == 0, what,
+  if (c10::hip::getCurrentHIPStream(like.get_device()).id() == 0) return;
+  auto check_stream = [&](Node* f) {
+    const auto s = f->stream();
+    NEED(!s || s->id() != 0, what,
          ": backward captured while an eager graph of the same leaf lives on the default stream: drop that graph, or capture with detached leaves");
+  };
+  const auto* exec = torch::autograd::get_current_graph_task_exec_info();      // (empty: a pass over everything)
+  std::unordered_set<Node*> seen;
+  std::vector<Node*> todo;
+  auto push = [&](const Node& f) {
+    for (const auto& e : f.next_edges()) {
+      Node* next = e.function.get();
+      if (!next) continue;
+      if (exec && !exec->empty()) {
+        const auto it = exec->find(next);
+        if (it == exec->end() || !it->second.should_execute()) continue;
+      }
+      if (seen.insert(next).second) todo.push_back(next);
+    }
+  };
+  for (const auto& e : n.next_edges())
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) check_stream(e.function.get());
+  push(n);
+  while (!todo.empty()) {
+    Node* f = todo.back();
+    todo.pop_back();
+    check_stream(f);
+    push(*f);
   }
 }
 Tensor empty(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape, like.options()); }

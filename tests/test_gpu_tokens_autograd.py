@@ -176,3 +176,34 @@ def test_tracing_is_refused():
         with pytest.raises(RuntimeError, match='traced'):
             torch.jit.trace(f, x, check_trace=False)
         f(x)
+
+
+# ---- captures --------------------------------------------------------------------------------------------------------------------------
+def test_captured_layer_beside_an_eager_graph_of_its_leaves_is_refused():
+    """the leaf's node is behind other operators (a projection, a split): refused all the same, and only where the captured pass would reach it"""
+    leaves, pos, kw, dims, go = _layer_inputs()
+    posd, god = pos.cuda(), go.cuda()
+    dl = [t.cuda().requires_grad_() for t in leaves]
+    alive = _layer(*dl, posd, kw, *dims)
+    want = torch.autograd.grad(alive, dl, god, retain_graph=True)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match='eager graph of the same leaf'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(_layer(*dl, posd, kw, *dims), dl, god)
+    gc.collect()
+    # another input of its own, the eager graph's projection not differentiated: nothing of the eager graph takes part
+    own = [t.detach().clone().requires_grad_() for t in dl[:3]] + [dl[3]]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            torch.autograd.grad(_layer(*own, posd, kw, *dims), own[:3], god)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(_layer(*own, posd, kw, *dims), own[:3], god)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, r) for a, r in zip(got, want))
+    assert all(torch.equal(a, r) for a, r in zip(torch.autograd.grad(alive, dl, god), want))
