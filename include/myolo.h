@@ -408,8 +408,10 @@ int myolo_detect_decode(const void* raw, int dtype, int n, int na, int ny, int n
  * What a transformer layer over feature-map tokens needs next to the 1x1 convolutions (the reference's is models/common.py:49-92). */
 
 /* Layer norm over the channels of every pixel row: y = (x - mu) * rstd * gamma + beta, rstd = (mean (x - mu)^2 + eps)^-1/2; statistics in
- * fp32.  x, out: views of one shape and dtype (any c >= 1, any strides; 16-byte aligned rows take the vector path); out may be x.
+ * fp32.  x, out: views of one shape and dtype (1 <= c <= MYOLO_LAYERNORM_MAX_C, any strides; 16-byte aligned rows take the vector path); out
+ * may be x.
  * gamma / beta: fp32[c] or NULL (1 / 0).  saved: fp32[2 * rows] (rows = n*h*w: the means, then the rstds) for the backward, or NULL. */
+#define MYOLO_LAYERNORM_MAX_C (1 << 29)
 int myolo_layernorm_fwd(const myolo_tensor* x, const float* gamma, const float* beta, float eps, const myolo_tensor* out, float* saved,
                         void* stream);
 /* gx (+)= rstd * (g - mean g - xhat * mean(g * xhat)), g = gout * gamma;  dgamma (+)= sum_rows gout * xhat;  dbeta (+)= sum_rows gout.
@@ -425,9 +427,10 @@ int myolo_layernorm_bwd(const myolo_tensor* gout, const myolo_tensor* x, const f
  * (2j, 2j + 1) when interleaved.  The turn count is formed and reduced in fp64.  inverse = 1: the opposite angle (the backward).
  * q [b, l, hq, d] and k [b, l, hk, d] share positions and launch; k == NULL (hk = 0): q alone.  qo / ko: the results; either is its
  * input itself (same strides) or does not overlap any input.  Strides in elements: {batch, token, head}, pos {batch, token, axis};
- * channel stride 1.  turns, axis: HOST arrays, read during the call. */
+ * channel stride 1.  turns, axis: HOST arrays, read during the call.  (hq + hk) * d <= MYOLO_ROPE_MAX_TOKEN. */
 #define MYOLO_ROPE_MAX_PAIRS 128
 #define MYOLO_ROPE_MAX_AXES 4
+#define MYOLO_ROPE_MAX_TOKEN (1 << 30)
 typedef struct myolo_rope_desc {
   const void *q, *k;
   void *qo, *ko;
@@ -441,7 +444,7 @@ int myolo_rope(const myolo_rope_desc* d, void* stream);
 
 /* Attention with a sliding window and leading keys that stay visible.  q, o [b, lq, hq, d], k, v [b, lk, hk, d] (hq a multiple of hk: query
  * head h reads key head h / (hq / hk)); element strides {batch, token, head}, channel stride 1.  d <= 128 and a multiple of 8, pointers
- * and strides multiples of 16 bytes, lq, lk, window <= MYOLO_ATTN_MAX_LEN, anything else is MYOLO_EINVAL.
+ * and strides multiples of 16 bytes, lq, lk, window <= MYOLO_ATTN_MAX_LEN, no launch of 2^32 threads or more; anything else is MYOLO_EINVAL.
  *   p = starts[b] + i  (starts == NULL: lk - lq + i) is query i's position;  key j is visible when  j < lens[b] (lens == NULL: lk)
  *   and (not causal or j <= p) and (window == 0 or |p - j| < window or j < sinks)
  *   o = softmax over the visible keys of scale * q.k, times v; a query that sees nothing gives 0.

@@ -919,6 +919,7 @@ int64_t key_span(const myolo_attn_desc* d, int rows) {
 }
 // workgroups of 256 threads that are resident at once: two a CU, one where a kernel's registers leave a SIMD one wave
 int resident(const myolo_attn_desc* d) { return d->dtype == MYOLO_F16 || d->d <= 64 ? 512 : 256; }
+bool fits(int64_t groups, int threads) { return groups * threads < (1ll << 32); }         // what one launch may hold
 struct FwdShape { int nw, nblk, nsplit; };
 FwdShape fwd_shape(const myolo_attn_desc* d) {
   const int64_t rows = (int64_t)d->lq * (d->hq / d->hk), bh = (int64_t)d->b * d->hk;
@@ -1070,7 +1071,7 @@ extern "C" int myolo_attn_fwd(const myolo_attn_desc* d, void* stream) {
   const FwdShape f = fwd_shape(d);
   AttnArgs a = args_of(d);
   a.nblk = f.nblk; a.nsplit = f.nsplit; a.part = (float*)d->ws;
-  if ((int64_t)a.b * a.hk * a.nblk * a.nsplit > 0x7fffffff) return MYOLO_EINVAL;
+  if (!fits((int64_t)a.b * a.hk * a.nblk * a.nsplit, f.nw * 64)) return MYOLO_EINVAL;
   if (f.nsplit > 1 && (!d->ws || (uintptr_t)d->ws % 16 || d->ws_bytes < myolo_attn_ws_bytes(d, 0))) return MYOLO_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   return d->dtype == MYOLO_F16 ? run_fwd<half_t>(a, f.nw, st) : run_fwd<float>(a, f.nw, st);
@@ -1088,10 +1089,11 @@ extern "C" int myolo_attn_bwd(const myolo_attn_desc* d, void* stream) {
   if (d->lq && (!d->ws || (uintptr_t)d->ws % 16 || d->ws_bytes < myolo_attn_ws_bytes(d, 1))) return MYOLO_EINVAL;
   AttnArgs a = args_of(d);
   const KvShape kv = kv_shape(d);
-  if ((int64_t)a.b * a.hk * ((a.rows + 127) / 128) > 0x7fffffff || (int64_t)a.b * a.hk * (kv.nblk + (int64_t)kv.nsb * kv.nsplit) > 0x7fffffff) return MYOLO_EINVAL;
+  a.nsplit = d->gq ? q_split(d) : 1;
+  if (!fits((int64_t)a.b * a.hk * ((a.rows + 127) / 128) * a.nsplit, 256) || !fits((int64_t)a.b * a.hk * (kv.nblk + (int64_t)kv.nsb * (kv.nsplit - 1)), 256))
+    return MYOLO_EINVAL;
   a.delta = (float*)d->ws;
   a.part = (float*)((char*)d->ws + delta_bytes(d));
-  a.nsplit = d->gq ? q_split(d) : 1;
   hipStream_t st = (hipStream_t)stream;
   return d->dtype == MYOLO_F16 ? run_bwd<half_t>(a, kv, st) : run_bwd<float>(a, kv, st);
 }

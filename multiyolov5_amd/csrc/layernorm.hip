@@ -384,23 +384,26 @@ __global__ __launch_bounds__(256) void ln_param_any_kernel(Rows go, Rows x, int6
 __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* ws, int n, int c, float* dgamma, float* dbeta, int acc) {
   __shared__ float sm[64][17];
   const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + cl;                  // 0 .. 2c: gamma's channels, then beta's
-  float s = 0.f;
-  if (col < 2 * c) {
+  for (int c0 = blockIdx.x * 16; c0 < 2 * c; c0 += gridDim.x * 16) {
+    const int col = c0 + cl;                             // 0 .. 2c: gamma's channels, then beta's
+    float s = 0.f;
+    if (col < 2 * c) {
 #pragma unroll 8
-    for (int i = sl; i < n; i += 64) s += ws[(int64_t)i * 2 * c + col];
-  }
-  sm[sl][cl] = s;
-  __syncthreads();
-  if (sl == 0 && col < 2 * c) {
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 64; ++i) s += sm[i][cl];
-    float* d = col < c ? dgamma : dbeta;
-    if (d) {
-      d += col < c ? col : col - c;
-      *d = acc ? *d + s : s;
+      for (int i = sl; i < n; i += 64) s += ws[(int64_t)i * 2 * c + col];
     }
+    sm[sl][cl] = s;
+    __syncthreads();
+    if (sl == 0 && col < 2 * c) {
+      s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 64; ++i) s += sm[i][cl];
+      float* d = col < c ? dgamma : dbeta;
+      if (d) {
+        d += col < c ? col : col - c;
+        *d = acc ? *d + s : s;
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -436,7 +439,7 @@ int bwd_groups(int64_t rows, const Lay& l) {
 }
 
 bool view_ok(const myolo_tensor& t) {
-  return (t.ptr || (int64_t)t.n * t.h * t.w == 0) && (t.dtype == MYOLO_F16 || t.dtype == MYOLO_F32) && t.n >= 0 && t.h >= 0 && t.w >= 0 && t.c >= 1 &&
+  return (t.ptr || (int64_t)t.n * t.h * t.w == 0) && (t.dtype == MYOLO_F16 || t.dtype == MYOLO_F32) && t.n >= 0 && t.h >= 0 && t.w >= 0 && t.c >= 1 && t.c <= MYOLO_LAYERNORM_MAX_C &&
          (int64_t)t.h * t.w < (1ll << 31) && (double)t.n * t.h * t.w < (double)(1ll << 40);
          // (rows of a map: 31 bits; all rows: 40)
 }
@@ -511,7 +514,7 @@ int ln_bwd(const myolo_tensor* gout, const myolo_tensor* x, const float* saved, 
     }
   }
   if (param) {
-    hipLaunchKernelGGL(ln_param_reduce_kernel, dim3((2 * c + 15) / 16), dim3(1024), 0, st, ws, ns, c, dgamma, dbeta, acc_params);
+    hipLaunchKernelGGL(ln_param_reduce_kernel, dim3(grid_for(2 * (int64_t)c, 16, 1 << 16)), dim3(1024), 0, st, ws, ns, c, dgamma, dbeta, acc_params);
     MYOLO_CHECK_LAUNCH();
   }
   return 0;

@@ -164,12 +164,13 @@ bool side_vec_ok(const RopeSide& s) {
 template <typename T> int run_rope(const RopeArgs& a, hipStream_t st) {
   constexpr int SEG = ET<T>::SEG;
   const int np = a.interleaved ? SEG / 2 : SEG, heads = a.s[0].h + a.s[1].h;
-  if (!(a.npair % np == 0 && (a.d - 2 * a.npair) % SEG == 0 && side_vec_ok(a.s[0]) && side_vec_ok(a.s[1]))) {
+  auto any = [&]() {
     const int grid = grid_for(a.tokens * heads * (a.d - a.npair), 256, 1 << 20);
     hipLaunchKernelGGL(rope_any_kernel<T>, dim3(grid), dim3(256), 0, st, a);
     MYOLO_CHECK_LAUNCH();
     return 0;
-  }
+  };
+  if (!(a.npair % np == 0 && (a.d - 2 * a.npair) % SEG == 0 && side_vec_ok(a.s[0]) && side_vec_ok(a.s[1]))) return any();
   const int units = a.npair / np, pass = (a.d - 2 * a.npair) / SEG, upt = units + pass;
   // four heads a thread where that still leaves sixteen waves for every CU, one where the call is that small
   const int hc = a.tokens * heads * upt >= 4 * 16 * 256 * 64 ? 4 : 1;
@@ -179,7 +180,8 @@ template <typename T> int run_rope(const RopeArgs& a, hipStream_t st) {
   if (tb > a.l) tb = a.l;
   while (tb > 1 && tb * a.npair > kTable) --tb;          // (npair <= 128: one token always fits)
   const int nb = (int)(a.tokens / a.l);
-  const dim3 grid((unsigned)((a.l + tb - 1) / tb), (unsigned)(nb < 65535 ? nb : 65535));
+  if ((a.l - 1) / tb >= (1 << 24) - 1) return any();     // (2^32 threads in one dimension)
+  const dim3 grid((unsigned)((a.l - 1) / tb + 1), (unsigned)(nb < 65535 ? nb : 65535));
 #define ROPE(IL, HC) hipLaunchKernelGGL((rope_vec_kernel<T, IL, HC>), grid, dim3(256), 0, st, a, units, pass, nq, nch, tb, nb)
   if (a.interleaved) { if (hc == 4) ROPE(true, 4); else ROPE(true, 1); }
   else { if (hc == 4) ROPE(false, 4); else ROPE(false, 1); }
@@ -197,6 +199,7 @@ extern "C" int myolo_rope(const myolo_rope_desc* d, void* stream) {
   if (d->naxis < 1 || d->naxis > MYOLO_ROPE_MAX_AXES) return MYOLO_EINVAL;
   for (int j = 0; j < d->npair; ++j)
     if (d->axis[j] < 0 || d->axis[j] >= d->naxis) return MYOLO_EINVAL;
+  if (((int64_t)d->hq + d->hk) * d->d > MYOLO_ROPE_MAX_TOKEN) return MYOLO_EINVAL;       // (items of a token are counted in 32 bits)
   const int64_t tokens = (int64_t)d->b * d->l;
   if (tokens == 0) return 0;
   if (!d->q || !d->qo || !d->pos || (d->hk && (!d->k || !d->ko))) return MYOLO_EINVAL;

@@ -222,7 +222,8 @@ struct LayerNormBackward : torch::autograd::Node {
 Tensor layer_norm(const Tensor& x_, const OptTensor& w_, const OptTensor& b_, double eps) {
   not_traced("layer_norm");
   const Tensor x = plain(x_, "layer_norm"), w = plain(of(w_), "layer_norm"), b = plain(of(b_), "layer_norm");
-  NEED(x.dim() > 0 && x.size(-1) >= 1 && x.size(-1) < (int64_t(1) << 31), "layer_norm: no channels in a tensor of shape ", x.sizes());
+  NEED(x.dim() > 0 && x.size(-1) >= 1, "layer_norm: no channels in a tensor of shape ", x.sizes());
+  NEED(x.size(-1) <= MYOLO_LAYERNORM_MAX_C, "layer_norm: ", x.size(-1), " channels (at most ", MYOLO_LAYERNORM_MAX_C, ")");
   NEED(eps >= 0.0 && std::isfinite(eps), "layer_norm: eps must be a number >= 0, got ", eps);
   for (const Tensor* p : {&w, &b})
     NEED(!p->defined() || (p->scalar_type() == at::kFloat && p->dim() == 1 && p->size(0) == x.size(-1) && p->is_cuda()),
@@ -332,7 +333,7 @@ std::pair<Tensor, OptTensor> rope_axes(const Tensor& q_, const OptTensor& k_, co
   NEED(!k.defined() || (k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3) && k.size(2) >= 1),
        "rope_axes: q ", q.sizes(), " and k ", k.sizes(), " differ in more than their heads");
   NEED(q.size(2) >= 1 && q.size(3) >= 1, "rope_axes: q ", q.sizes());
-  for (int i = 0; i < 4; ++i) NEED(q.size(i) < (int64_t(1) << 31), "rope_axes: q ", q.sizes());
+  for (int i = 0; i < 4; ++i) NEED(q.size(i) < (int64_t(1) << 31) && (!k.defined() || k.size(i) < (int64_t(1) << 31)), "rope_axes: q ", q.sizes(), " is too large");
   NEED(2 * npair <= q.size(3) && npair <= MYOLO_ROPE_MAX_PAIRS, "rope_axes: ", npair, " pairs in ", q.size(3), " channels (at most ", MYOLO_ROPE_MAX_PAIRS, ")");
   NEED((pos.dim() == 2 || pos.dim() == 3) && pos.size(-2) == q.size(1) && pos.size(-1) == naxis &&
            (pos.dim() == 2 || pos.size(0) == 1 || pos.size(0) == q.size(0)),

@@ -51,7 +51,7 @@ def _tensor(t, what, dtype=None, dim=None):
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """(x - mean) * (var + eps)^-1/2 * weight + bias over the last dimension of x [..., C] (any C >= 1, any strides; a channels-last feature
+    """(x - mean) * (var + eps)^-1/2 * weight + bias over the last dimension of x [..., C] (1 <= C <= 2^29, any strides; a channels-last feature
     map is x.permute(0, 2, 3, 1)).  weight, bias: fp32 [C] or None.  The result is contiguous, in x's dtype; gradients for x, weight, bias."""
     _tensor(x, 'layer_norm: x')
     return _ext().layer_norm(x, weight, bias, eps)
@@ -66,6 +66,8 @@ def rope_table(sections, theta=10000.0, spectrum='shared'):
     if spectrum not in ('shared', 'axis') or not 0.0 < theta < math.inf:
         raise L.MyoloError(f'rope_axes: spectrum {spectrum!r}, theta {theta!r}')
     n = sum(sections)
+    if n > L.ROPE_MAX_PAIRS:
+        raise L.MyoloError(f'rope_axes: {n} rotary pairs (at most {L.ROPE_MAX_PAIRS})')
     turns, axis = [], []
     for a, na in enumerate(sections):
         for j in range(na):
