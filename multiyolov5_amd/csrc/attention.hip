@@ -279,10 +279,13 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
 
   const char* kp = a.k + b * a.ks[0] + kh * a.ks[2];
   const char* vp = a.v + b * a.vs[0] + kh * a.vs[2];
+  // fp16 probabilities enter the product as 2^11 .. 2^15 times what they are of the largest: what thousands of weak keys add up to would be lost
+  // in subnormals otherwise (40000 keys of 2^-26 each: all of it).  A key's is off by at most 2^-36 now: half a step of a result for 2^25 keys
+  constexpr float kLift = sizeof(T) == 2 ? 11.f : 0.f, kSlack = sizeof(T) == 2 ? 4.f : 8.f;
   f16_t o[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) o[m] = f16_t{};
-  float mx = -INFINITY, l = 0.f;
+  float mx = -INFINITY, l = 0.f;              // the reference the probabilities are formed with (log2), their sum
 
   const TileList tl = tiles_of(vis, pb0, pb1, BK);
   const Keys bkeys = vis.keys(pb0, pb1), lkeys = vis.keys(p, p);       // the workgroup's keys, the lane's
@@ -340,10 +343,10 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) m2 = fmaxf(m2, s[u][r]);
-      // the reference maximum follows the running one only when that has outgrown it by 2^8 (in fp16 a probability may be that large): after the
-      // first tiles the sums are hardly ever rescaled
-      m2 = half_max(m2) * a.sl2;
-      if (__any(m2 > mx + 8.f)) {
+      // the reference lies kLift under the maximum it was taken from and follows the running one only when that has outgrown it by kSlack: the sums are
+      // hardly ever rescaled after the first tiles
+      m2 = half_max(m2) * a.sl2 - kLift;
+      if (__any(m2 > mx + kSlack)) {
         m2 = fmaxf(mx, m2);
         const float al = __builtin_amdgcn_exp2f(mx - (m2 == -INFINITY ? 0.f : m2));
         mx = m2;
