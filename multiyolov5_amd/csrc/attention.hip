@@ -536,8 +536,17 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // The forward's walk with the two score products formed again per tile: seven products in all instead of the five of one fused pass, whose dq would
 // need atomics or a pass over partial sums of every key block.  2 x 4096, window 1024, 16 / 4 heads x 128 fp16: 158 us, 570 TFLOP/s of its
 // three products; bound like the forward.
-// P enters the fp16 products times 2^12: a probability below 6e-5 (rows of more than 2^14 keys) would lose bits as an fp16 subnormal
-constexpr float kPShift = 12.f, kPUnshift = 1.f / 4096.f;
+// P enters the fp16 product of dv times 2^12: a probability below 6e-5 (rows of more than 2^14 keys) would lose bits as an fp16 subnormal.
+// dS has the size of P times the incoming gradient, anything from 1e-8 (a mean over a map's pixels) to more than the largest half: it enters
+// its products times a power of two, the query's own in dq, the key's own in dk.  That starts at 2^24 and falls, with the sums formed so far,
+// whenever an element would pass 2^15, to where the largest lies between 2^7 and 2^8: beside its relative half step an element is off by 2^-32 of
+// the largest seen at most.  64 queries x 8192 keys, gradients of 1e-4: gq off by 7.2 % with dS as it is, by 0.93 % so, which is its own rounding;
+// 16 x 2048 tokens of 64 channels cost 205 -> 215 us a pass for it, 2 x 4096 of 128 channels 526 -> 537.
+template <typename T> constexpr float kPShift = sizeof(T) == 2 ? 12.f : 0.f;
+template <typename T> constexpr float kPUnshift = sizeof(T) == 2 ? 1.f / 4096.f : 1.f;
+constexpr int kMostUp = 24;
+constexpr float kTop = 32768.f;
+__device__ __forceinline__ int to_room(float m) { return 134 - (int)(__float_as_uint(m) >> 23); }       // 2^that * m lies in [2^7, 2^8), m > 0
 
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
@@ -584,6 +593,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
   const int64_t lrow = ((int64_t)b * a.hq + head) * a.lq + qi;
   const float lse = a.lse[lrow];
   if (live && h == 0 && sp == 0) a.delta[lrow] = delta;
+  constexpr bool kUp = sizeof(T) == 2;
+  int up = kUp ? kMostUp : 0;                                // the exponent that dS and dq are lifted by
+  float nl = live ? (float)up - lse : -INFINITY;
   const char* kp = a.k + b * a.ks[0] + kh * a.ks[2];
   const char* vp = a.v + b * a.vs[0] + kh * a.vs[2];
   f16_t dq[MT];
@@ -639,10 +651,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
         Columns<T, DL, kAhead> ck(sK, u * 32, lane);
         ck.first();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, -lse)) * (dp[r] - delta);
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, nl)) * (dp[r] - delta);
         if (!all) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = lkeys.has(j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? s[r] : 0.f;
+        }
+        if constexpr (kUp) {
+          float top = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[r]));
+          if (__builtin_expect(__any(top > kTop), 0)) {
+            top = half_max(top);
+            const int e = top > kTop ? to_room(top) : 0;
+            const float f = __builtin_amdgcn_ldexpf(1.f, e);
+            up += e;
+            nl = live ? (float)up - lse : -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= f;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) dq[m][r] *= f;
+          }
         }
         Frag<T> d0, d1;
         frag_from<0>(d0, s);
@@ -660,6 +690,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
     if (more) put();
   }
   if (!live || !a.gq) return;
+  const float down = __builtin_amdgcn_ldexpf(a.nsplit > 1 ? 1.f : a.scale, -up);
   if (a.nsplit > 1) {
     float* po = a.part + (((int64_t)sp * (a.b * a.hk) + bh) * a.rows + row) * a.d;
 #pragma unroll
@@ -667,7 +698,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const int c = m * 32 + q4 * 8 + 4 * h;
-        if (c < a.d) *reinterpret_cast<f4_t*>(po + c) = f4_t{dq[m][4 * q4], dq[m][4 * q4 + 1], dq[m][4 * q4 + 2], dq[m][4 * q4 + 3]};
+        if (c < a.d) *reinterpret_cast<f4_t*>(po + c) = f4_t{dq[m][4 * q4], dq[m][4 * q4 + 1], dq[m][4 * q4 + 2], dq[m][4 * q4 + 3]} * down;
       }
     return;
   }
@@ -677,7 +708,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int c = m * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
-      if (c < a.d) reinterpret_cast<T*>(dp)[c] = (T)(dq[m][r] * a.scale);
+      if (c < a.d) reinterpret_cast<T*>(dp)[c] = (T)(dq[m][r] * down);
     }
 }
 
@@ -744,6 +775,9 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_
   f16_t dk[MT], dv[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) dk[m] = dv[m] = f16_t{};
+  constexpr bool kUp = sizeof(T) == 2;
+  int up = kUp ? kMostUp - (int)kPShift<T> : 0;              // what 2^kPShift dS and dk of the lane's key are lifted by
+  float upf = __builtin_amdgcn_ldexpf(1.f, up);
 
   Stage<T, DP, BQ, NT> gq, gg;
   float nl = 0.f, nd = 0.f;
@@ -756,8 +790,8 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_
     if (tid < BQ) {
       const bool on = ok(tid);
       const int64_t lr = ((int64_t)b * a.hq + head) * a.lq + (on ? i0 + tid : 0);
-      nl = on ? kPShift - a.lse[lr] : 0.f;
-      nd = on ? a.delta[lr] * kPUnshift : 0.f;
+      nl = on ? kPShift<T> - a.lse[lr] : 0.f;
+      nd = on ? -a.delta[lr] : 0.f;
     }
   };
   auto put = [&]() {
@@ -828,10 +862,39 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_
         frag_from<0>(f0, s);
         frag_from<1>(f1, s);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = s[r] * fmaf(dp[r], kPUnshift, -d4[r >> 2][r & 3]);
+        for (int r = 0; r < 16; ++r) dp[r] = s[r] * (dp[r] + d4[r >> 2][r & 3]);
         if (!all) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) dp[r] = lrows.has(p0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) ? dp[r] : 0.f;
+        }
+        if constexpr (kUp) {
+          float top = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dp[r]));
+          if (__builtin_expect(__any(top * upf > kTop), 0)) {
+            // (held where the matrix instructions keep them up to here: else the allocator copies all of dk out for this branch in every step)
+            if constexpr (DP > 64) {
+#pragma unroll
+              for (int m = 0; m < MT; ++m) asm("" : "+a"(dk[m]));
+            }
+            top = half_max(top);
+            const int to = top * upf > kTop ? to_room(top) : up;
+            const float f = __builtin_amdgcn_ldexpf(1.f, to - up);
+            up = to;
+            upf = __builtin_amdgcn_ldexpf(1.f, up);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {                   // (the sums' rows are keys, other lanes' own)
+              const float fr = __shfl(f, (r & 3) + 8 * (r >> 2) + 4 * h, 64);
+#pragma unroll
+              for (int m = 0; m < MT; ++m) dk[m][r] *= fr;
+            }
+            if constexpr (DP > 64) {
+#pragma unroll
+              for (int m = 0; m < MT; ++m) asm("" : "+a"(dk[m]));
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] *= upf;
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -856,6 +919,15 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_
   }
   // accumulators: column (lane % 32) = channel, rows = keys
   const int col = lane & 31;
+  if constexpr (kUp) {
+    const float down = __builtin_amdgcn_ldexpf(kPUnshift<T>, -up);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float dr = __shfl(down, (r & 3) + 8 * (r >> 2) + 4 * h, 64);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) dk[m][r] *= dr;
+    }
+  }
   if (part) {
     float* pk = a.part + (((int64_t)bh * a.nsb + blk) * a.nsplit + sp) * (2 * 32 * NW) * a.d;
     float* pv = pk + 32 * NW * a.d;
@@ -875,7 +947,7 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_
       const int kk = kw0 + (r & 3) + 8 * (r >> 2) + 4 * h;
       if (kk < a.lk && m * 32 + col < a.d) {
         reinterpret_cast<T*>(a.gk + b * a.gks[0] + kh * a.gks[2] + (int64_t)kk * a.gks[1])[m * 32 + col] = (T)(dk[m][r] * a.scale);
-        reinterpret_cast<T*>(a.gv + b * a.gvs[0] + kh * a.gvs[2] + (int64_t)kk * a.gvs[1])[m * 32 + col] = (T)(dv[m][r] * kPUnshift);
+        reinterpret_cast<T*>(a.gv + b * a.gvs[0] + kh * a.gvs[2] + (int64_t)kk * a.gvs[1])[m * 32 + col] = (T)(dv[m][r] * kPUnshift<T>);
       }
     }
 }
@@ -894,7 +966,7 @@ __global__ __launch_bounds__(256) void attn_bwd_kv_join_kernel(AttnArgs a) {
     f4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = 0; i < a.nsplit; ++i) s += *reinterpret_cast<const f4_t*>(p + (int64_t)i * 2 * 128 * a.d);
-    const float f = which ? kPUnshift : a.scale;
+    const float f = which ? kPUnshift<T> : a.scale;
     T* g = which ? (T*)(a.gv + b * a.gvs[0] + kh * a.gvs[2] + (int64_t)kk * a.gvs[1]) : (T*)(a.gk + b * a.gks[0] + kh * a.gks[2] + (int64_t)kk * a.gks[1]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) g[c + e] = (T)(s[e] * f);
