@@ -207,3 +207,101 @@ def test_captured_layer_beside_an_eager_graph_of_its_leaves_is_refused():
         torch.cuda.synchronize()
         assert all(torch.equal(a, r) for a, r in zip(got, want))
     assert all(torch.equal(a, r) for a, r in zip(torch.autograd.grad(alive, dl, god), want))
+
+
+# ---- layers in launch plans ------------------------------------------------------------------------------------------------------------
+def test_attn_layer_with_frozen_parts():
+    """no gradient for the input; frozen parameters stay without one and change nothing for the others"""
+    from multiyolov5_amd.models.common import AttnLayer
+    torch.manual_seed(0)
+    m = AttnLayer(32, 2, 1, 2, 3).cuda().train()
+    x, go = rnd(1, 2, 32, 5, 7).cuda(), rnd(2, 2, 32, 5, 7).cuda()
+    m(x.clone().requires_grad_()).backward(go)
+    want = {k: p.grad.clone() for k, p in m.named_parameters()}
+    m.zero_grad(set_to_none=True)
+    m(x).backward(go)
+    for k, p in m.named_parameters():
+        assert float((p.grad - want[k]).norm()) <= 1e-5 * float(want[k].norm()), k
+    m.zero_grad(set_to_none=True)
+    m.norm1.weight.requires_grad_(False)
+    m.qkv.bias.requires_grad_(False)
+    m(x).backward(go)
+    for k, p in m.named_parameters():
+        if p.requires_grad:
+            assert float((p.grad - want[k]).norm()) <= 1e-5 * float(want[k].norm()), k
+        else:
+            assert p.grad is None, k
+
+
+def test_attn_layer_repeats_once_its_plans_are_captured():
+    """launch lists run eagerly at first and as graphs from the third pass on: the same gradients, and those of other inputs in between"""
+    from multiyolov5_amd.models.common import AttnLayer
+    torch.manual_seed(0)
+    m = AttnLayer(64, 4, 2, 2, 3).cuda().train()
+    first = {}
+    for i in range(9):
+        x, go = rnd(i % 2, 2, 64, 9, 12).cuda().requires_grad_(), rnd(10 + i % 2, 2, 64, 9, 12).cuda()
+        m.zero_grad(set_to_none=True)
+        y = m(x)
+        y.backward(go)
+        got = [y.detach().clone(), x.grad] + [p.grad.clone() for p in m.parameters()]
+        want = first.setdefault(i % 2, got)
+        for a, r in zip(got, want):
+            assert float((a - r).norm()) <= 1e-5 * float(r.norm()), i
+
+
+def test_attn_layer_in_half_follows_its_weights():
+    """the fp32 copies of a half model's norm weights are formed again when the weights change"""
+    from multiyolov5_amd.models.common import AttnLayer
+    torch.manual_seed(0)
+    m = AttnLayer(32, 2, 2, 1, 1).cuda().eval().half()
+    x = rnd(1, 1, 32, 6, 8, dt=F16).cuda()
+    with torch.no_grad():
+        for step in range(3):
+            for _ in range(4):
+                y = m(x).clone()
+            m32 = AttnLayer(32, 2, 2, 1, 1).cuda().eval()
+            m32.load_state_dict({k: v.float() for k, v in m.state_dict().items()})
+            r = m32(x.float())
+            assert float((y.float() - r).norm()) <= 2e-2 * float(r.norm()), step
+            m.norm1.weight.mul_(1.5)
+            m.norm2.bias.add_(0.7)
+        m.float()                                                        # and back: parameters that were allocated again
+        assert float((m(x.float()) - m32.cuda().train(False)(x.float())).norm()) > 0
+        m32.load_state_dict(m.state_dict())
+        r = m32(x.float())
+        assert float((m(x.float()) - r).norm()) <= 1e-5 * float(r.norm())
+
+
+# ---- threads ---------------------------------------------------------------------------------------------------------------------------
+def test_calls_of_several_threads():
+    """passes of four threads at once, each on a stream of its own, give what one thread gives"""
+    import threading
+    leaves, pos, kw, dims, go = _layer_inputs()
+    posd, god = pos.cuda(), go.cuda()
+
+    def once(k):
+        l = [(t * (1 + k)).cuda().requires_grad_() for t in leaves]
+        o = _layer(*l, posd, kw, *dims)
+        return [o.detach(), *torch.autograd.grad(o, l, god)]
+    want = [once(k) for k in range(4)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(25):
+                    got = once(k)
+                    s.synchronize()
+                    if not all(torch.equal(a, r) for a, r in zip(got, want[k])):
+                        bad.append(k)
+        except Exception as e:                                           # noqa: BLE001
+            bad.append(e)
+    ts = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad, bad
