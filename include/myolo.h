@@ -449,7 +449,7 @@ int myolo_rope(const myolo_rope_desc* d, void* stream);
  *   and (not causal or j <= p) and (window == 0 or |p - j| < window or j < sinks)
  *   o = softmax over the visible keys of scale * q.k, times v; a query that sees nothing gives 0.
  * Keys that no query of the call sees, and queries that see nothing, are never read into a result, whatever they hold; a NaN or infinity in any
- * other row may reach the results of rows within 64 tokens of it.  lens, starts: device int32[b].
+ * other row may reach results up to 128 tokens beyond the mask, and the gradients of the 31 keys behind the sinks.  lens, starts: device int32[b].
  * lse: fp32 [b, hq, lq] (log2 of the softmax denominator of scale*log2(e)*q.k), written by the forward when not NULL, read by the
  * backward.  o_res (fp16, laid out like o; may be NULL, NULL for fp32): what the rounding of o left over, written by the forward, read by the
  * backward, whose row sums of go * o would otherwise carry o's rounding into gq and gk.  scale > 0.

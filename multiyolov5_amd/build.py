@@ -45,10 +45,10 @@ def stale():
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-# augment.hip restates C code compiled for baseline x86-64 (Pillow / OpenCV float arithmetic): a fused multiply-add changes the
-# truncated uint8 results.  hipcc's default -ffp-contract=fast ignores source pragmas, so the whole file is built without contraction.
 # no v_pk_{add,mul,fma}_f32 anywhere: scalar fp32 instructions give the same IEEE results
 NO_PACKED_F32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+# augment.hip restates C code compiled for baseline x86-64 (Pillow / OpenCV float arithmetic): a fused multiply-add changes the
+# truncated uint8 results.  hipcc's default -ffp-contract=fast ignores source pragmas, so the whole file is built without contraction.
 PER_FILE_FLAGS = {'augment.hip': ['-ffp-contract=off']}
 
 

@@ -253,8 +253,8 @@ __device__ __forceinline__ int xcd_order(int id, int n) {
 // ---- forward -------------------------------------------------------------------------------------------------------------------------
 // A workgroup takes 128 rows (four waves x 32) through its key tiles, or 32 rows in one wave where the call has no more (one token: the key
 // axis is split over workgroups).  Bound by the matrix pipe and the softmax's vector instructions in turn, two waves a SIMD covering each
-// other: causal 8192 x 128 channels, 32 / 8 heads fp16 in 0.61 ms, 900 TFLOP/s (pipe 43 % busy); 64 channels have half the products for the same
-// softmax: 16 x 2048, window 256 both ways, 4 heads in 51 us, 320 TFLOP/s.  One token over 8 caches of up to 32768 x 8 heads x 128: 138 us, 5.9 TB/s,
+// other: causal 8192 x 128 channels, 32 / 8 heads fp16 in 0.65 ms, 850 TFLOP/s (pipe 43 % busy); 64 channels have half the products for the same
+// softmax: 16 x 2048, window 256 both ways, 4 heads in 49 us, 330 TFLOP/s.  One token over 8 caches of up to 32768 x 8 heads x 128: 151 us, 5.3 TB/s,
 // bound by HBM.
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, NW == 4 && (sizeof(T) == 2 || DP <= 64) ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
@@ -534,7 +534,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 // ---- backward: dq (and delta) --------------------------------------------------------------------------------------------------------
 // The forward's walk with the two score products formed again per tile: seven products in all instead of the five of one fused pass, whose dq would
-// need atomics or a pass over partial sums of every key block.  2 x 4096, window 1024, 16 / 4 heads x 128 fp16: 158 us, 570 TFLOP/s of its
+// need atomics or a pass over partial sums of every key block.  2 x 4096, window 1024, 16 / 4 heads x 128 fp16: 171 us, 530 TFLOP/s of its
 // three products; bound like the forward.
 // P enters the fp16 product of dv times 2^12: a probability below 6e-5 (rows of more than 2^14 keys) would lose bits as an fp16 subnormal.
 // dS has the size of P times the incoming gradient, anything from 1e-8 (a mean over a map's pixels) to more than the largest half: it enters
@@ -733,8 +733,8 @@ __global__ __launch_bounds__(256) void attn_bwd_q_join_kernel(AttnArgs a) {
 // A wave owns 32 keys (operands and both accumulators in registers); the workgroup's four waves walk the query tiles that may see its 128
 // keys, once for every head of the group: the gradient of a shared head is one sum in one place.  Blocks that hold sinks see every query,
 // and few blocks leave CUs idle: blocks [0, nsb) share their walk between nsplit workgroups, whose partial sums a second kernel adds in
-// a fixed order.  128 channels hold 420 registers, one wave a SIMD: 2 x 4096, window 1024, 16 / 4 heads fp16 in 237 us, 510 TFLOP/s of its four products,
-// a third of the time waiting; 64 channels run two waves: 16 x 2048, window 256 both ways, 4 heads in 83 us, 390 TFLOP/s, bound by issue slots.
+// a fixed order.  128 channels hold 420 registers, one wave a SIMD: 2 x 4096, window 1024, 16 / 4 heads fp16 in 256 us, 470 TFLOP/s of its four products,
+// a third of the time waiting; 64 channels run two waves: 16 x 2048, window 256 both ways, 4 heads in 90 us, 360 TFLOP/s, bound by issue slots.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
   constexpr bool kAhead = kAheadOf<T>;

@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void ln_bwd_any_kernel(Rows go, Rows x, Rows g
 // ---- rows held in registers ----------------------------------------------------------------------------------------------------------
 // A row belongs to G adjacent lanes (4 .. 64 of a wave, or the whole workgroup of 256), each holding NV vectors of it: x and gout are read once,
 // their next row is in flight while this one is reduced and written, gamma / beta and the parameter sums stay in registers over all rows
-// of a workgroup.  HBM bound: 131072 rows of 192 fp16 channels forward 21.5 us (4.7 TB/s), backward 36 us (4.2 TB/s; 74 % of the vector
+// of a workgroup.  HBM bound: 131072 rows of 192 fp16 channels forward 21.6 us (4.7 TB/s), backward 34 us (4.4 TB/s; 74 % of the vector
 // unit's issue slots), 4 us for the parameter sums; 4097 rows of 1003 fp32 channels, element by element, 9 and 20 us.
 template <typename T, int VEC, int NV> struct RowRegs {
   uint4 raw[VEC > 1 ? NV : 1];

@@ -57,8 +57,8 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a) {
 // Vector path: a workgroup owns tb tokens.  It forms their sines and cosines once, in LDS, for all heads, behind the loads of what they will
 // turn: a thread owns one 16-byte unit of pairs (SEG pairs (j, j + npair) in two vectors, or SEG / 2 neighbouring pairs in one) of HC heads of
 // q or of k.  Adjacent lanes take adjacent units, then other heads of the token: HBM sees whole lines.  Units behind the pairs copy the
-// pass-through channels.  HBM bound: 35154 tokens x 16 heads x 96 fp32 in 74 us (5.8 TB/s; 121 with the angles formed by every thread),
-// 32768 tokens x 16 heads x 64 fp16 in 27 us (4.9 TB/s); one token of 40 heads 3.5 us.
+// pass-through channels.  HBM bound: 35154 tokens x 16 heads x 96 fp32 in 77 us (5.6 TB/s; 121 with the angles formed by every thread),
+// 32768 tokens x 16 heads x 64 fp16 in 30 us (4.4 TB/s); one token of 40 heads 3.9 us.
 template <typename T, bool IL, int HC> struct RopeItem {
   static constexpr int SEG = ET<T>::SEG, NP = IL ? SEG / 2 : SEG, NV = IL ? 1 : 2;
   uint4 in[HC][NV];

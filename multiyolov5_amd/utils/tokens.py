@@ -102,7 +102,8 @@ def window_attention(q, k, v, window=0, sinks=0, causal=False, lens=None, starts
     visible however far the window has moved.  lens, starts: int32 [B] on the device (a padded batch; a cache longer than what it holds).
     A query that sees nothing gives zeros and takes no gradient.  What keys hold that no query of the call sees, and queries that see nothing,
     does not matter; everything else has to be finite: a NaN in a key that some queries see, or in a query that sees some keys, may also reach
-    the results of its neighbours (64 tokens), as 0 * NaN does in a product of masked probabilities.  scale: default D^-1/2, > 0.
+    results up to 128 tokens beyond the mask, and the gradients of the 31 keys behind the sinks, as 0 * NaN does in a product of masked
+    probabilities.  scale: default D^-1/2, > 0.
     One new token over a long cache is split over the key axis.  Gradients for q, k and v, formed without atomics (a run repeats bit for bit)."""
     _tensor(q, 'window_attention: q', dim=4)
     _tensor(k, 'window_attention: k', q.dtype, 4)
