@@ -106,3 +106,19 @@ def test_many_keys_of_little_weight(lq, lk, h):
     assert float((bound / ref).max()) < 0.2
     o = T().window_attention(q.cuda(), k.cuda(), v.cuda(), scale=1.0)
     R.within('o', o, ref, bound)
+
+
+@pytest.mark.parametrize('d', [24, 48, 64, 80, 96, 128])
+@pytest.mark.parametrize('b,hk,causal', [(1, 1, False), (20, 6, True)])
+def test_score_gradients_that_climb_from_tile_to_tile(d, b, hk, causal):
+    """incoming gradients that grow from query tile to query tile, values that grow from key tile to key tile, each by its own factor: the lift of every
+    query and key falls again and again with sums formed before (few blocks: split walks; many: whole ones)"""
+    n, h = 330, 2 * hk
+    q, k, v, go = (rnd(30 + i, b, n, m, d) for i, m in enumerate((h, hk, hk, h)))
+    tile = torch.arange(n) // 64
+    go = (go.float() * 2.0 ** (4.0 * tile - 12)[None, :, None, None]).to(F16)
+    v = (v.float() * 2.0 ** (3.0 * tile - 9)[None, :, None, None]).to(F16)
+    kw = dict(causal=causal)
+    ref = R.attention(q, k, v, go=go, **kw)
+    assert all(float(ref[name][0].abs().max()) < 6e4 for name in ref)
+    against(q, k, v, go, 1.0, **kw)
